@@ -549,6 +549,8 @@ void dpb_shutdown(dpb_ctx* ctx) {
     cudaFree(ctx->counter);
     cudaFree(ctx->stage_dev);
     cudaFreeHost(ctx->result_host);
+    if (ctx->fwd_host) cudaFreeHost(ctx->fwd_host);
+    if (ctx->fwd_words) cudaFree(ctx->fwd_words);
     cudaEventDestroy(ctx->prof_ev[0]);
     cudaEventDestroy(ctx->prof_ev[1]);
     cudaStreamDestroy(ctx->stream);

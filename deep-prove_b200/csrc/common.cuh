@@ -171,6 +171,12 @@ struct dpb_ctx {
     // tests: challenges posted to a resident kernel so far, and the one that is held back (dpb_resident_hold)
     uint64_t tail_posts = 0, tail_hold_post = ~0ull;
     uint32_t tail_hold_ms = 0;
+    // forward operators (forward.cuh), made on first use: the word their value checks publish for the host and the
+    // word a kernel that gave up waiting leaves behind (mapped), and the checks' counters on the device
+    void* fwd_host = nullptr;
+    void* fwd_dev = nullptr;
+    unsigned int* fwd_words = nullptr;
+    unsigned int fwd_seq = 0;
     // optional per-kernel timing log (dpb_profile_enable)
     bool profile = false;
     cudaEvent_t prof_ev[2] = {nullptr, nullptr};

@@ -1,0 +1,74 @@
+// What the forward operators' translation units share: the check that a kernel makes of its input values and the host
+// waits for, and the handle of rows sorted by key.
+#pragma once
+#include "common.cuh"
+
+struct dpb_row_groups {
+    dpb_ctx* ctx = nullptr;
+    uint64_t n = 0, n_keys = 0;
+    void* block = nullptr;
+    uint32_t* keys = nullptr;     // the keys, ascending
+    uint32_t* rows = nullptr;     // the row at each place of that order
+    uint32_t* offsets = nullptr;  // first place of every key (n_keys + 1 entries); null beyond kGroupOffsets keys
+};
+
+namespace dpb {
+
+constexpr uint32_t kGroupOffsets = 4095;  // with the end, one tile of the counting sort's scan
+
+enum FwdError : unsigned int { kFwdKeyRange = 1, kFwdValueRange = 2 };
+
+// How a kernel tells the host what it thinks of its input: the checking blocks or their findings into `words[0]`, the
+// last of them (a ticket in words[1]) publishes {findings, sequence number} in mapped memory as one 8-byte store and
+// clears the words for the next launch.  The host polls the sequence number, which saves the wait for the kernel's end
+// and for whatever was queued behind it.
+struct FwdCheck {
+    unsigned int* words;
+    uint2* status;  // mapped
+    unsigned int seq;
+};
+__device__ __forceinline__ void fwd_publish(const FwdCheck& c, unsigned int found) {
+    __threadfence_system();
+    *(volatile unsigned long long*)c.status = ((unsigned long long)c.seq << 32) | found;
+}
+// Called by every thread of each of the `blocks` checking blocks, once, after its checks; `found` is the thread's.
+__device__ __forceinline__ void fwd_check_done(const FwdCheck& c, unsigned int found, unsigned int blocks) {
+    const unsigned int any = (unsigned)__syncthreads_or((int)found);  // the findings' bits are told apart below
+    if (any && found) atomicOr(c.words, found);
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        if (atomicAdd(c.words + 1, 1u) == blocks - 1) {
+            const unsigned int all = atomicExch(c.words, 0u);
+            c.words[1] = 0;
+            fwd_publish(c, all);
+        }
+    }
+}
+
+// Restores the caller's current device (the context's own may be another).
+struct FwdDevice {
+    int before = -1;
+    cudaError_t err;
+    explicit FwdDevice(const dpb_ctx* ctx) {
+        err = cudaGetDevice(&before);
+        if (err == cudaSuccess && before != ctx->device) err = cudaSetDevice(ctx->device);
+    }
+    ~FwdDevice() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+// The next check of the context (api_forward.cu); DPB_ETIMEOUT when a kernel of an earlier call gave up waiting.
+int fwd_check_begin(dpb_ctx* ctx, FwdCheck* out);
+// Waits (bounded) for the check's findings.
+int fwd_check_wait(dpb_ctx* ctx, const FwdCheck& c, unsigned int* found);
+// The word in mapped memory a kernel that gives up waiting sets (device address).
+unsigned int* fwd_gave_up_word(dpb_ctx* ctx);
+// A host tensor's copy on the device (*owned, to be freed after the launches), or the device tensor itself.  The host
+// buffer may be reused once the stream has passed the copy: fwd_check_wait behind it, or a synchronisation.
+int fwd_tensor(dpb_ctx* ctx, const int64_t* src, int on_device, uint64_t numel, const int64_t** dev, void** owned);
+
+inline uint64_t pow2_ceil(uint64_t x) { return 1ull << log2u(x); }
+
+}  // namespace dpb

@@ -1,0 +1,405 @@
+// Integer matrix products grouped by expert, on the tensor cores' 8-bit integer form.
+//
+// y = x W exactly, |x| < 2^14, |W| < 2^14: both sides are cut into signed 8-bit digits, x = x0 + 256 x1 (one digit when
+// 8 bits suffice), and the products of digits are added up in 32-bit integers by tcgen05.mma kind::i8, one accumulator
+// per power of 256:  acc0 = W0 x0,  acc1 = W0 x1 + W1 x0,  acc2 = W1 x1;  y = acc0 + 2^8 acc1 + 2^16 acc2 in 64 bits.
+// A digit product is at most 2^14 in magnitude and acc1 takes two per step, so up to 2^15 steps stay below 2^31
+// (kMaxSteps); a longer inner dimension is cut, like a short list of tiles, over several work items that add their
+// 64-bit results to the output (exact, so their order does not matter).
+//
+// The weights' 128 columns are the instruction's M (rows of the accumulator = TMEM lanes) and a tile's routed rows its
+// N: a warp's lanes then hold neighbouring columns of one output row, which is stored as whole 256-byte runs without a
+// transposition, and a tile of few rows (a single token) wastes nothing.
+#pragma once
+#include "forward.cuh"
+
+struct dpb_expert_weights {
+    dpb_ctx* ctx = nullptr;
+    uint32_t n_experts = 0, bits = 0, digits = 0;
+    uint64_t inner = 0, cols = 0;
+    uint32_t col_tiles = 0, k_blocks = 0;
+    int8_t* planes = nullptr;  // [expert][column tile][128 of the inner dimension][digit][128 columns x 128 bytes]
+};
+
+namespace dpb {
+
+constexpr uint32_t kTileCols = 128, kTileK = 128;  // weight columns per tile; inner entries per stage (bytes of a digit)
+constexpr uint32_t kTileBytes = kTileCols * kTileK;
+constexpr uint32_t kMaxSteps = 256;  // stages per work item: 2^15 inner entries
+
+// A tile's digits lie as the instruction reads them with the 128-byte swizzle: row r's 128 bytes at r * 128, the
+// 16-byte pieces of a row exchanged by xor with r mod 8.  One copy then brings a whole tile, with no tensor map.
+__device__ __forceinline__ uint32_t tile_piece(uint32_t row, uint32_t piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+
+// 16 values -> 16-byte pieces of their digits; whether all lie in range
+template <int DIGITS>
+__device__ __forceinline__ bool cut_digits(const int64_t (&x)[16], int64_t half, uint4 (&out)[DIGITS]) {
+    uint32_t w[DIGITS][4];
+    bool ok = true;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t d0 = 0, d1 = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int64_t v = x[4 * i + j];
+            ok = ok && v >= -half && v < half;
+            const int lo = (int)(int8_t)v;
+            d0 |= (uint32_t)(uint8_t)lo << (8 * j);
+            if (DIGITS == 2) d1 |= (uint32_t)(uint8_t)(((int)v - lo) >> 8) << (8 * j);
+        }
+        w[0][i] = d0;
+        if (DIGITS == 2) w[DIGITS - 1][i] = d1;
+    }
+#pragma unroll
+    for (int d = 0; d < DIGITS; d++) out[d] = make_uint4(w[d][0], w[d][1], w[d][2], w[d][3]);
+    return ok;
+}
+
+// Weights [expert][inner][cols] -> planes.  A thread takes 16 inner entries of one column: neighbouring threads read
+// neighbouring columns.  Made once per model.
+constexpr uint32_t kCutThreads = 256;
+template <int DIGITS>
+__global__ void __launch_bounds__(kCutThreads)
+    cut_weights_kernel(const int64_t* __restrict__ w, uint32_t n_experts, uint64_t inner, uint64_t cols, uint32_t col_tiles,
+                       uint32_t k_blocks, int64_t half, int8_t* __restrict__ planes, FwdCheck check) {
+    unsigned int found = 0;
+    const uint64_t padded = (uint64_t)col_tiles * kTileCols, pieces = (uint64_t)k_blocks * 8;
+    const uint64_t total = n_experts * pieces * padded;
+    for (uint64_t t = (uint64_t)blockIdx.x * kCutThreads + threadIdx.x; t < total; t += (uint64_t)gridDim.x * kCutThreads) {
+        const uint64_t c = t % padded, q = t / padded, piece = q % pieces, e = q / pieces;
+        int64_t x[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const uint64_t k = piece * 16 + i;
+            x[i] = c < cols && k < inner ? w[(e * inner + k) * cols + c] : 0;
+        }
+        uint4 d[DIGITS];
+        if (!cut_digits<DIGITS>(x, half, d)) found = kFwdValueRange;
+        const uint64_t tile = (e * col_tiles + c / kTileCols) * k_blocks + piece / 8;
+#pragma unroll
+        for (int i = 0; i < DIGITS; i++)
+            *(uint4*)(planes + (tile * DIGITS + i) * kTileBytes + tile_piece(c % kTileCols, piece % 8)) = d[i];
+    }
+    fwd_check_done(check, found, gridDim.x);
+}
+
+// first tile of every expert: tiles[e] = sum of ceil(rows / T) over the experts before e
+__device__ __forceinline__ void expert_tiles(const uint32_t* __restrict__ offsets, uint32_t n_experts, uint32_t rows_log2,
+                                             uint32_t* tiles /* shared, n_experts + 1 */) {
+    const uint32_t T1 = (1u << rows_log2) - 1;
+    if (threadIdx.x < 32) {
+        uint32_t carry = 0;
+        for (uint32_t e0 = 0; e0 < n_experts; e0 += 32) {
+            const uint32_t e = e0 + threadIdx.x;
+            const uint32_t n = e < n_experts ? (offsets[e + 1] - offsets[e] + T1) >> rows_log2 : 0;
+            uint32_t incl = n;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const uint32_t u = __shfl_up_sync(0xffffffffu, incl, off);
+                if (threadIdx.x >= (uint32_t)off) incl += u;
+            }
+            if (e < n_experts) tiles[e] = carry + incl - n;
+            carry += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (threadIdx.x == 0) tiles[n_experts] = carry;
+    }
+}
+
+// Routed rows in sorted order -> planes [row tile][128 of the inner dimension][digit][T rows x 128 bytes].  A thread cuts
+// 16 entries of a row.  Rows of a tile past the expert's last are left as they are: their products are not stored.
+template <int DIGITS>
+__global__ void __launch_bounds__(kCutThreads)
+    cut_rows_kernel(const int64_t* __restrict__ x, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ rows,
+                    const uint32_t* __restrict__ offsets, uint64_t n, uint32_t per, uint32_t n_experts, uint64_t inner,
+                    uint32_t k_blocks, uint32_t rows_log2, int64_t half, int8_t* __restrict__ planes, FwdCheck check) {
+    extern __shared__ uint32_t tiles[];
+    unsigned int found = 0;
+    expert_tiles(offsets, n_experts, rows_log2, tiles);
+    __syncthreads();
+    const uint32_t pieces = k_blocks * 8, T = 1u << rows_log2;
+    const uint64_t total = n * pieces;
+    const bool aligned = (inner & 1) == 0 && ((uintptr_t)x & 15) == 0;
+    for (uint64_t t = (uint64_t)blockIdx.x * kCutThreads + threadIdx.x; t < total; t += (uint64_t)gridDim.x * kCutThreads) {
+        const uint64_t p = t / pieces;
+        const uint32_t piece = (uint32_t)(t - p * pieces), e = keys[p];
+        if (e >= n_experts) continue;
+        const int64_t* src = x + (uint64_t)(rows[p] / per) * inner + piece * 16;
+        const uint64_t left = inner > piece * 16 ? inner - piece * 16 : 0;
+        int64_t v[16];
+        if (aligned && left >= 16) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) *(longlong2*)(v + i) = __ldg((const longlong2*)(src + i));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] = i < left ? __ldg(src + i) : 0;
+        }
+        uint4 d[DIGITS];
+        if (!cut_digits<DIGITS>(v, half, d)) found = kFwdValueRange;
+        const uint32_t at = (uint32_t)p - offsets[e];
+        const uint64_t tile = (uint64_t)(tiles[e] + (at >> rows_log2)) * k_blocks + piece / 8;
+#pragma unroll
+        for (int i = 0; i < DIGITS; i++)
+            *(uint4*)(planes + (tile * DIGITS + i) * (T * 128) + tile_piece(at & (T - 1), piece & 7)) = d[i];
+    }
+    fwd_check_done(check, found, gridDim.x);
+}
+
+// ------------------------------------------------------------------------------------------------ PTX
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Waits for the phase; gives up (and tells the block's other roles) after kWaitTries tries, seconds at the least.
+constexpr uint32_t kWaitTries = 1u << 24;
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+    for (uint32_t i = 0; i < kWaitTries; i++) {
+        if (bar_try(bar, parity)) return true;
+        if (*gave_up) return false;
+    }
+    *gave_up = 1;
+    return false;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar) : "memory");
+}
+// shared-memory operand, K-major, 128-byte swizzle: 8-row groups 1024 bytes apart
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+           ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a),
+                 "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// 16 columns of the warp's 32 lanes
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
+
+// ------------------------------------------------------------------------------------------------ the product
+struct GroupedArgs {
+    const int8_t* weights;
+    const int8_t* x;
+    const uint32_t* offsets;
+    const uint32_t* rows;
+    uint32_t n_experts, col_tiles, k_blocks;
+    uint32_t splits, blocks_per_split;  // work items along the inner dimension, and their stages
+    uint64_t cols;
+    int64_t* out;
+    unsigned int* gave_up;
+};
+
+// XD, WD: digits of x and of the weights; T: rows per tile.
+template <int XD, int WD, int T>
+struct GroupedShape {
+    static constexpr int kAcc = XD + WD - 1;
+    static constexpr uint32_t kStageBytes = WD * kTileBytes + XD * T * 128;
+    static constexpr uint32_t kStages = 216 * 1024 / kStageBytes < 8 ? 216 * 1024 / kStageBytes : 8;
+    static constexpr int kBuffers = 2 * kAcc * T <= 512 ? 2 : 1;  // accumulators: the next tile's while one is stored
+    static constexpr uint32_t kCols = kBuffers * kAcc * T;
+    static constexpr uint32_t kTmem = kCols <= 32 ? 32 : kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+    static constexpr uint32_t smem(uint32_t n_experts) { return kStages * kStageBytes + 1024 + (n_experts + 1) * 4; }
+};
+
+// Six warps: 0-3 move finished accumulators to the output, 4 brings the operands, 5 issues the products.  One block per
+// SM walks the work items blockIdx.x, + gridDim.x, ...; items of one expert are ordered with the row tiles fastest, so
+// that the blocks at work at one time share the weights' and rows' tiles in L2.
+template <int XD, int WD, int T>
+__global__ void __launch_bounds__(192, 1) grouped_product_kernel(GroupedArgs a) {
+    typedef GroupedShape<XD, WD, T> S;
+    constexpr uint32_t rows_log2 = T == 16 ? 4 : T == 32 ? 5 : T == 64 ? 6 : 7;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[2 * S::kStages + 4];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int gave_up;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ring = (smem_addr(smem_raw) + 1023) & ~1023u;
+    uint32_t* tiles = (uint32_t*)(smem_raw + (ring - smem_addr(smem_raw)) + S::kStages * S::kStageBytes);
+    const uint32_t bar0 = smem_addr(bars);
+    auto full = [&](uint32_t s) { return bar0 + 8 * s; };
+    auto empty = [&](uint32_t s) { return bar0 + 8 * (S::kStages + s); };
+    auto acc_full = [&](uint32_t b) { return bar0 + 8 * (2 * S::kStages + b); };
+    auto acc_empty = [&](uint32_t b) { return bar0 + 8 * (2 * S::kStages + 2 + b); };
+    expert_tiles(a.offsets, a.n_experts, rows_log2, tiles);
+    if (threadIdx.x == 0) {
+        gave_up = 0;
+        for (uint32_t s = 0; s < S::kStages; s++) {
+            bar_init(full(s), 1);
+            bar_init(empty(s), 1);
+        }
+        for (uint32_t b = 0; b < 2; b++) {
+            bar_init(acc_full(b), 1);
+            bar_init(acc_empty(b), 4);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(S::kTmem)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+    const uint64_t per_tile = (uint64_t)a.col_tiles * a.splits, items = tiles[a.n_experts] * per_tile;
+
+    // the item's expert (found by walking on from the last item's), its row tile, column tile and stages
+    struct Item {
+        uint32_t expert, row_tile, col_tile, first, last;
+    };
+    auto item_at = [&](uint64_t i, uint32_t& e) {
+        while (i >= tiles[e + 1] * per_tile) e++;
+        const uint32_t mine = tiles[e + 1] - tiles[e];
+        const uint64_t j = i - tiles[e] * per_tile;
+        Item it;
+        it.expert = e;
+        it.row_tile = (uint32_t)(j % mine);
+        const uint32_t q = (uint32_t)(j / mine);
+        it.col_tile = q % a.col_tiles;
+        it.first = q / a.col_tiles * a.blocks_per_split;
+        it.last = it.first + a.blocks_per_split < a.k_blocks ? it.first + a.blocks_per_split : a.k_blocks;
+        return it;
+    };
+
+    uint32_t e = 0;
+    if (warp == 4 && lane == 0) {
+        uint32_t stage = 0, phase = 0;
+        for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {
+            const Item it = item_at(i, e);
+            const int8_t* w = a.weights + ((uint64_t)(e * a.col_tiles + it.col_tile) * a.k_blocks) * (WD * kTileBytes);
+            const int8_t* x = a.x + ((uint64_t)(tiles[e] + it.row_tile) * a.k_blocks) * (XD * T * 128);
+            for (uint32_t k = it.first; k < it.last; k++) {
+                if (!bar_wait(empty(stage), phase ^ 1, &gave_up)) goto done;
+                const uint32_t dst = ring + stage * S::kStageBytes;
+                bar_expect(full(stage), S::kStageBytes);
+                bulk_load(dst, w + (uint64_t)k * (WD * kTileBytes), WD * kTileBytes, full(stage));
+                bulk_load(dst + WD * kTileBytes, x + (uint64_t)k * (XD * T * 128), XD * T * 128, full(stage));
+                if (++stage == S::kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+        // the last products release their stages before the block may end
+        for (uint32_t s = 0; s < S::kStages; s++) {
+            if (!bar_wait(empty(stage), phase ^ 1, &gave_up)) goto done;
+            if (++stage == S::kStages) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
+    } else if (warp == 5 && lane == 0) {
+        // D = S32, A and B = signed 8 bits, both K-major
+        constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(T >> 3) << 17) | ((kTileCols >> 4) << 24);
+        uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
+        for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {
+            const Item it = item_at(i, e);
+            if (!bar_wait(acc_empty(buf), buf_phase ^ 1, &gave_up)) goto done;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t acc = tmem + buf * (S::kAcc * T);
+            for (uint32_t k = it.first; k < it.last; k++) {
+                if (!bar_wait(full(stage), phase, &gave_up)) goto done;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t base = ring + stage * S::kStageBytes;
+#pragma unroll
+                for (int wd = 0; wd < WD; wd++)
+#pragma unroll
+                    for (int xd = 0; xd < XD; xd++)
+#pragma unroll
+                        for (int s = 0; s < (int)kTileK / 32; s++) {
+                            // the first product into an accumulator overwrites it: digit pairs (0, 0), (0, 1) or (1, 0), (1, 1)
+                            const bool first = s == 0 && (wd == 0 || xd == XD - 1);
+                            mma_i8(acc + (wd + xd) * T, operand_desc(base + wd * kTileBytes + s * 32),
+                                   operand_desc(base + WD * kTileBytes + xd * (T * 128) + s * 32), idesc, !(first && k == it.first));
+                        }
+                mma_commit(empty(stage));
+                if (++stage == S::kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            mma_commit(acc_full(buf));
+            if (++buf == S::kBuffers) {
+                buf = 0;
+                buf_phase ^= 1;
+            }
+        }
+    } else if (warp < 4) {
+        uint32_t buf = 0, buf_phase = 0;
+        for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {
+            const Item it = item_at(i, e);
+            if (!bar_wait(acc_full(buf), buf_phase, &gave_up)) goto done;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t lo = a.offsets[e] + it.row_tile * T, end = a.offsets[e + 1];
+            const int valid = end - lo < T ? (int)(end - lo) : T;
+            const uint64_t c = (uint64_t)it.col_tile * kTileCols + warp * 32 + lane;
+            const uint32_t acc = tmem + buf * (S::kAcc * T) + (warp << 21);
+            for (int j0 = 0; j0 < valid; j0 += 16) {
+                uint32_t r[S::kAcc][16];
+#pragma unroll
+                for (int d = 0; d < S::kAcc; d++) tmem_load16(acc + d * T + j0, r[d]);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (j0 + 16 >= valid) {  // the accumulators are in registers: the next tile's products may start
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(acc_empty(buf));
+                }
+                if (c < a.cols) {
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        if (j0 + j >= valid) break;
+                        int64_t y = (int32_t)r[0][j];
+#pragma unroll
+                        for (int d = 1; d < S::kAcc; d++) y += (int64_t)(int32_t)r[d][j] << (8 * d);
+                        int64_t* o = a.out + (uint64_t)a.rows[lo + j0 + j] * a.cols + c;
+                        if (a.splits > 1) atomicAdd((unsigned long long*)o, (unsigned long long)y);
+                        else __stcs((long long*)o, (long long)y);
+                    }
+                }
+            }
+            if (++buf == S::kBuffers) {
+                buf = 0;
+                buf_phase ^= 1;
+            }
+        }
+    }
+done:
+    __syncwarp();
+    __syncthreads();
+    if (gave_up) {
+        // copies and products in flight must not outlive the block: wait for every stage that was asked for, with a limit
+        if (threadIdx.x == 0) {
+            *(volatile unsigned int*)a.gave_up = 1;
+            for (uint32_t t = 0; t < (1u << 20); t++) __nanosleep(1000);
+        }
+        __syncthreads();
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kTmem));
+    }
+}
+
+}  // namespace dpb

@@ -1,0 +1,112 @@
+"""Python face of include/dpb_forward.h: the forward operators that make the integer tensors the provers take, and their
+transposes.  Device tensors are (table, shape) pairs, as Context.upload_tensor_i64 returns them; results of that form can
+be handed to the einsum and lookup calls' device_tensor arguments."""
+import ctypes
+
+import numpy as np
+
+from . import FR_I64, Mle, _buf, _int, _pp, _u32, _u64, _vp, check, lib
+
+_i64 = ctypes.c_int64
+FORWARD_SIGNATURES = {
+    "dpb_embedding_lookup": (_int, [_vp, _vp, _u64, _u64, _u64, _vp, _int, _u64, _i64, _u32, _int, _pp]),
+    "dpb_row_groups_new": (_int, [_vp, _vp, _int, _u64, _u64, _pp]),
+    "dpb_row_groups_len": (_u64, [_vp]),
+    "dpb_row_groups_free": (None, [_vp]),
+    "dpb_row_groups_sum": (_int, [_vp, _vp, _int, _vp, _vp, _int, _u64, _u32, _i64, _pp]),
+    "dpb_expert_weights_new": (_int, [_vp, _vp, _int, _u32, _u64, _u64, _u32, _pp]),
+    "dpb_expert_weights_free": (None, [_vp]),
+    "dpb_grouped_product": (_int, [_vp, _int, _vp, _vp, _int, _u32, _u32, _vp, _pp]),
+}
+for _name, (_res, _args) in FORWARD_SIGNATURES.items():
+    _fn = getattr(lib, _name)
+    _fn.restype = _res
+    _fn.argtypes = _args
+
+
+def _source(array, device):
+    """(pointer, 1 when on the device, shape, what must stay alive) of an int64 tensor given either way."""
+    if device is not None:
+        mle, shape = device
+        return ctypes.c_void_p(lib.dpb_mle_device_ptr(mle.h)), 1, tuple(shape), mle
+    a = np.ascontiguousarray(array, dtype=np.int64)
+    return _buf(a), 0, a.shape, a
+
+
+def _pow2(n):
+    return 1 << (max(int(n), 1) - 1).bit_length()
+
+
+def embedding_lookup(ctx, table, vocab, width, tokens, multiplier=1, right_shift=0, row_stride=None, padded=False,
+                     device_tokens=None):
+    """dpb_embedding_lookup: the rows of `tokens`, rescaled.  `table`: an integer table of vocab rows, row_stride
+    (default: width) entries apart.  Returns (table, shape): the [n, width] tensor, or with padded=True the table of
+    the padded shape."""
+    ptr, on_device, shape, _keep = _source(tokens, device_tokens)
+    n = int(np.prod(shape, dtype=np.int64))
+    h = ctypes.c_void_p()
+    check(lib.dpb_embedding_lookup(ctx.h, table.h, vocab, width, width if row_stride is None else row_stride, ptr, on_device, n,
+                                   multiplier, right_shift, 1 if padded else 0, ctypes.byref(h)))
+    return Mle(ctx, h), (_pow2(n), _pow2(width)) if padded else (n, width)
+
+
+class RowGroups:
+    """dpb_row_groups: rows sorted by key (tokens, or the expert of every routed row)."""
+
+    def __init__(self, ctx, keys, n_keys, device_keys=None):
+        self.ctx, self.h = ctx, None
+        ptr, on_device, shape, _keep = _source(keys, device_keys)
+        self.n, self.n_keys = int(np.prod(shape, dtype=np.int64)), int(n_keys)
+        h = ctypes.c_void_p()
+        check(lib.dpb_row_groups_new(ctx.h, ptr, on_device, self.n, n_keys, ctypes.byref(h)))
+        self.h = h
+
+    def sums(self, family_dtype, weights=None, rows=None, rows_per_token=1, multiplier=1, device_rows=None):
+        """dpb_row_groups_sum: out[k, c] = multiplier * sum over rows i with key k of weights[i] * rows[i //
+        rows_per_token, c], a table of the padded shape over the family's challenge elements."""
+        if rows is None and device_rows is None:
+            ptr, on_device, width = None, 0, 1
+        else:
+            ptr, on_device, shape, _keep = _source(rows, device_rows)
+            if len(shape) != 2 or shape[0] < -(-self.n // rows_per_token):
+                raise ValueError(f"rows of shape {shape} for {self.n} keys, {rows_per_token} per token")
+            width = shape[1]
+        h = ctypes.c_void_p()
+        check(lib.dpb_row_groups_sum(self.ctx.h, self.h, family_dtype, weights.h if weights is not None else None, ptr, on_device,
+                                     width, rows_per_token, multiplier, ctypes.byref(h)))
+        return Mle(self.ctx, h)
+
+    def free(self):
+        if self.h:
+            lib.dpb_row_groups_free(self.h)
+            self.h = None
+
+
+class ExpertWeights:
+    """dpb_expert_weights: [expert, in, out] integers of at most `bits` bits, laid out for grouped_product."""
+
+    def __init__(self, ctx, weights, bits, device_weights=None):
+        self.ctx, self.h = ctx, None
+        ptr, on_device, shape, _keep = _source(weights, device_weights)
+        if len(shape) != 3:
+            raise ValueError(f"weights of shape {shape}: [expert, in, out] expected")
+        self.n_experts, self.inner, self.cols = (int(d) for d in shape)
+        h = ctypes.c_void_p()
+        check(lib.dpb_expert_weights_new(ctx.h, ptr, on_device, self.n_experts, self.inner, self.cols, bits, ctypes.byref(h)))
+        self.h = h
+
+    def free(self):
+        if self.h:
+            lib.dpb_expert_weights_free(self.h)
+            self.h = None
+
+
+def grouped_product(ctx, groups, x, x_bits, weights, rows_per_token=1, device_x=None, family_dtype=FR_I64):
+    """dpb_grouped_product: row i of x[i // rows_per_token] times its expert's matrix, exact.  Returns (table, shape) of
+    the [rows, out] tensor, rows in the order of the groups' keys."""
+    ptr, on_device, shape, _keep = _source(x, device_x)
+    if len(shape) != 2 or shape[1] != weights.inner or shape[0] * rows_per_token != groups.n:
+        raise ValueError(f"x of shape {shape} for {groups.n} routed rows, {rows_per_token} per token, of {weights.inner} entries")
+    h = ctypes.c_void_p()
+    check(lib.dpb_grouped_product(ctx.h, family_dtype, groups.h, ptr, on_device, x_bits, rows_per_token, weights.h, ctypes.byref(h)))
+    return Mle(ctx, h), (groups.n, weights.cols)
