@@ -36,7 +36,7 @@ int fwd_check_begin(dpb_ctx* ctx, FwdCheck* out) {
         return fail(DPB_ETIMEOUT, "a kernel of an earlier forward call gave up waiting; that call's result is not valid");
     }
     out->words = ctx->fwd_words;
-    out->status = (uint2*)ctx->fwd_dev;
+    out->status = (unsigned long long*)ctx->fwd_dev;
     out->seq = ++ctx->fwd_seq;
     return DPB_OK;
 }
@@ -77,9 +77,14 @@ int fwd_tensor(dpb_ctx* ctx, const int64_t* src, int on_device, uint64_t numel, 
 }
 
 template <class T, int V>
-static void launch_lookup(dpb_ctx* ctx, const LookupArgs& a, bool check_all, uint32_t blocks) {
-    if (check_all) embedding_lookup_kernel<T, V, true><<<blocks, kLookupThreads, 0, ctx->stream>>>(a);
-    else embedding_lookup_kernel<T, V, false><<<blocks, kLookupThreads, 0, ctx->stream>>>(a);
+static void launch_lookup(dpb_ctx* ctx, const LookupArgs& a, bool check_all, bool index32, uint32_t blocks) {
+    if (index32) {
+        if (check_all) embedding_lookup_kernel<T, V, true, uint32_t><<<blocks, kLookupThreads, 0, ctx->stream>>>(a);
+        else embedding_lookup_kernel<T, V, false, uint32_t><<<blocks, kLookupThreads, 0, ctx->stream>>>(a);
+    } else {
+        if (check_all) embedding_lookup_kernel<T, V, true, uint64_t><<<blocks, kLookupThreads, 0, ctx->stream>>>(a);
+        else embedding_lookup_kernel<T, V, false, uint64_t><<<blocks, kLookupThreads, 0, ctx->stream>>>(a);
+    }
 }
 
 static int lookup_impl(dpb_ctx* ctx, const dpb_mle* table, uint64_t vocab, uint64_t width, uint64_t stride, const int64_t* tokens,
@@ -124,14 +129,15 @@ static int lookup_impl(dpb_ctx* ctx, const dpb_mle* table, uint64_t vocab, uint6
     const int V = i32 ? 4 : 2;
     const bool vec = a.out_width % V == 0 && stride % V == 0 && ((uintptr_t)table->ptr & 15) == 0 && vocab * stride <= table->len;
     const uint64_t steps = a.out_rows * ((a.out_width + (vec ? V : 1) - 1) / (vec ? V : 1));
-    const uint32_t blocks = (uint32_t)std::min<uint64_t>((steps + kLookupThreads - 1) / kLookupThreads, (uint64_t)ctx->sm_count * 8);
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>((steps + kLookupThreads - 1) / kLookupThreads, (uint64_t)ctx->sm_count * 4);
+    const bool index32 = steps + (uint64_t)kLookupFlight * blocks * kLookupThreads < (1ull << 32);
     a.check_blocks = check_all ? 0 : (uint32_t)std::min<uint64_t>(blocks, (n + 8 * kLookupThreads - 1) / (8 * kLookupThreads));
     if (i32) {
-        if (vec) launch_lookup<int32_t, 4>(ctx, a, check_all, blocks);
-        else launch_lookup<int32_t, 1>(ctx, a, check_all, blocks);
+        if (vec) launch_lookup<int32_t, 4>(ctx, a, check_all, index32, blocks);
+        else launch_lookup<int32_t, 1>(ctx, a, check_all, index32, blocks);
     } else {
-        if (vec) launch_lookup<int64_t, 2>(ctx, a, check_all, blocks);
-        else launch_lookup<int64_t, 1>(ctx, a, check_all, blocks);
+        if (vec) launch_lookup<int64_t, 2>(ctx, a, check_all, index32, blocks);
+        else launch_lookup<int64_t, 1>(ctx, a, check_all, index32, blocks);
     }
     const cudaError_t e = cudaGetLastError();
     unsigned int found = 0;
@@ -153,12 +159,13 @@ static int groups_impl(dpb_ctx* ctx, const int64_t* keys, int on_device, dpb_row
     const uint32_t n = (uint32_t)g->n, n_keys = (uint32_t)g->n_keys;
     const bool small = n <= kSmallSort, dense = n_keys <= kGroupOffsets;
     const uint32_t counters = n_keys + 1, tiles = (counters + kCountTile - 1) / kCountTile;
-    // one block: [keys | rows | offsets or counters (+ tile sums, ranks)]
+    // one block: [keys | rows | places | offsets or counters]
     auto up = [](uint64_t words) { return (words + 63) & ~63ull; };
-    const uint64_t w_rows = up(n), w_off = w_rows + up(n), w_end = w_off + (dense || !small ? up((uint64_t)counters + 1) : 0);
+    const uint64_t w_rows = up(n), w_places = 2 * up(n), w_off = 3 * up(n), w_end = w_off + (dense || !small ? up((uint64_t)counters + 1) : 0);
     DPB_TRY(device_alloc(ctx, (w_end ? w_end : 1) * 4, &g->block));
     g->keys = (uint32_t*)g->block;
     g->rows = g->keys + w_rows;
+    g->places = g->keys + w_places;
     uint32_t* counts = g->keys + w_off;
     if (dense) g->offsets = counts;
     if (n == 0) {
@@ -173,13 +180,14 @@ static int groups_impl(dpb_ctx* ctx, const int64_t* keys, int on_device, dpb_row
     int rc = DPB_OK;
     cudaError_t e = cudaSuccess;
     if (small) {
-        const uint32_t n_pow2 = (uint32_t)std::max<uint64_t>(pow2_ceil(n), 2);
-        groups_small_kernel<<<1, kSmallSortThreads, 0, ctx->stream>>>(dev, n, n_keys, n_pow2, g->keys, g->rows, g->offsets, check);
+        const uint32_t probes = n + (dense ? n_keys + 1 : 0), per_block = kSmallSortThreads / 8;
+        groups_small_kernel<<<(probes + per_block - 1) / per_block, kSmallSortThreads, ((n + 31) & ~31u) * 4, ctx->stream>>>(
+            dev, n, n_keys, g->keys, g->rows, g->places, g->offsets, check);
         e = cudaGetLastError();
     } else {
-        rc = device_alloc(ctx, (up(n) + up(tiles)) * 4, &scratch);
+        rc = device_alloc(ctx, tiles * 4, &scratch);
         if (rc == DPB_OK) {
-            uint32_t *rank = (uint32_t*)scratch, *tile_sums = rank + up(n);
+            uint32_t *rank = g->places, *tile_sums = (uint32_t*)scratch;
             e = cudaMemsetAsync(counts, 0, (uint64_t)counters * 4, ctx->stream);
             if (e == cudaSuccess) {
                 groups_count_kernel<<<grid_for(ctx, n), kThreads, 0, ctx->stream>>>(dev, n, n_keys, counts, rank, check);
@@ -228,7 +236,7 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
     cudaError_t e = cudaSuccess;
     int rc = DPB_OK;
     if (!rows) {
-        a.slice = 512;
+        a.slice = kKeySumSlice;
         const uint64_t slices = (a.n + a.slice - 1) / a.slice;
         const uint32_t key_blocks = (uint32_t)((out_keys + kKeySumThreads - 1) / kKeySumThreads);
         if (slices > 1) rc = device_alloc(ctx, slices * 2 * sizeof(E), &parts);
@@ -246,10 +254,10 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
         }
     } else {
         rc = fwd_tensor(ctx, rows, rows_on_device, (a.n + per - 1) / per * width, &a.x, &owned);
-        const uint64_t col_blocks = (width + kRowSumThreads - 1) / kRowSumThreads;
-        // slices of at least 64 rows, and no more of them than fill the GPU some times over
-        const uint64_t want = std::max<uint64_t>(1, (uint64_t)ctx->sm_count * 16 / col_blocks);
-        a.slice = std::max<uint64_t>(kRowSumBatch, (a.n + want - 1) / want);
+        const uint64_t per_block = weights ? 2 * kRowSumThreads : kRowSumThreads, col_blocks = (width + per_block - 1) / per_block;
+        // slices of at least 16 rows, and no more of them than fill the GPU some times over
+        const uint64_t want = std::min<uint64_t>(65535, std::max<uint64_t>(1, (uint64_t)ctx->sm_count * 8 / col_blocks));
+        a.slice = std::max<uint64_t>(16, (a.n + want - 1) / want);
         const uint64_t slices = (a.n + a.slice - 1) / a.slice;
         if (rc == DPB_OK && slices > 1) rc = device_alloc(ctx, slices * 2 * width * sizeof(E), &parts);
         if (rc == DPB_OK) {
@@ -257,9 +265,12 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
             e = cudaMemsetAsync(m->ptr, 0, m->len * sizeof(E), ctx->stream);  // keys without rows, and the padding
             if (e == cudaSuccess && a.n) {
                 const dim3 grid((uint32_t)col_blocks, (uint32_t)slices);
-                if (weights) row_sums_kernel<F, true><<<grid, kRowSumThreads, 0, ctx->stream>>>(a, scale, scaled);
-                else row_sums_kernel<F, false><<<grid, kRowSumThreads, 0, ctx->stream>>>(a, scale, scaled);
-                if (slices > 1) row_sums_join_kernel<F><<<grid, kRowSumThreads, 0, ctx->stream>>>(a, scale, scaled);
+                if (weights) row_products_kernel<F><<<grid, kRowSumThreads, 0, ctx->stream>>>(a, scale, scaled);
+                else row_sums_kernel<F><<<grid, kRowSumThreads, 0, ctx->stream>>>(a, scale, scaled);
+                if (slices > 1) {
+                    const dim3 join((uint32_t)((width + kRowSumThreads - 1) / kRowSumThreads), (uint32_t)slices);
+                    row_sums_join_kernel<F><<<join, kRowSumThreads, 0, ctx->stream>>>(a, scale, scaled);
+                }
                 e = cudaGetLastError();
             }
         }

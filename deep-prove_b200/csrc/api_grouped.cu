@@ -78,15 +78,15 @@ static int product_impl(dpb_ctx* ctx, int dtype, const dpb_row_groups* g, const 
     cudaError_t e = cudaSuccess;
     unsigned int found = 0;
     if (rc == DPB_OK) {
-        const uint64_t pieces = n * w->k_blocks * 8;
-        const uint32_t blocks = (uint32_t)std::min<uint64_t>((pieces + kCutThreads - 1) / kCutThreads, (uint64_t)ctx->sm_count * 8);
+        const uint64_t cuts = n / per * ((w->k_blocks + 1) / 2), per_block = kCutThreads / 32;
+        const uint32_t blocks = (uint32_t)std::min<uint64_t>((cuts + per_block - 1) / per_block, (uint64_t)ctx->sm_count * 8);
         const size_t smem = (w->n_experts + 1) * 4;
         const int64_t half = 1ll << (x_bits - 1);
         if (digits == 1)
-            cut_rows_kernel<1><<<blocks, kCutThreads, smem, ctx->stream>>>(dev, g->keys, g->rows, g->offsets, n, per, w->n_experts, w->inner,
+            cut_rows_kernel<1><<<blocks, kCutThreads, smem, ctx->stream>>>(dev, g->keys, g->places, g->offsets, n / per, per, w->n_experts, w->inner,
                                                                            w->k_blocks, rows_log2, half, (int8_t*)planes, check);
         else
-            cut_rows_kernel<2><<<blocks, kCutThreads, smem, ctx->stream>>>(dev, g->keys, g->rows, g->offsets, n, per, w->n_experts, w->inner,
+            cut_rows_kernel<2><<<blocks, kCutThreads, smem, ctx->stream>>>(dev, g->keys, g->places, g->offsets, n / per, per, w->n_experts, w->inner,
                                                                            w->k_blocks, rows_log2, half, (int8_t*)planes, check);
         e = cudaGetLastError();
         GroupedArgs a;

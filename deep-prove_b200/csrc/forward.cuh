@@ -9,6 +9,7 @@ struct dpb_row_groups {
     void* block = nullptr;
     uint32_t* keys = nullptr;     // the keys, ascending
     uint32_t* rows = nullptr;     // the row at each place of that order
+    uint32_t* places = nullptr;   // the place of each row
     uint32_t* offsets = nullptr;  // first place of every key (n_keys + 1 entries); null beyond kGroupOffsets keys
 };
 
@@ -20,42 +21,40 @@ enum FwdError : unsigned int { kFwdKeyRange = 1, kFwdValueRange = 2 };
 
 // How a kernel tells the host what it thinks of its input: the checking blocks or their findings into `words[0]`, the
 // last of them (a ticket in words[1]) publishes {findings, sequence number} in mapped memory as one 8-byte store and
-// clears the words for the next launch.  The host polls the sequence number, which saves the wait for the kernel's end
-// and for whatever was queued behind it.
+// clears the words for the next launch; a single checking block publishes at once.  The host polls the sequence number,
+// which saves the wait for the kernel's end and for whatever was queued behind it.  Nothing else is published, so the
+// store needs no fence: results are ordered by the stream.
 struct FwdCheck {
     unsigned int* words;
-    uint2* status;  // mapped
+    unsigned long long* status;  // mapped
     unsigned int seq;
 };
-__device__ __forceinline__ void fwd_publish(const FwdCheck& c, unsigned int found) {
-    __threadfence_system();
-    *(volatile unsigned long long*)c.status = ((unsigned long long)c.seq << 32) | found;
-}
 // Called by every thread of each of the `blocks` checking blocks, once, after its checks; `found` is the thread's.
 __device__ __forceinline__ void fwd_check_done(const FwdCheck& c, unsigned int found, unsigned int blocks) {
-    const unsigned int any = (unsigned)__syncthreads_or((int)found);  // the findings' bits are told apart below
-    if (any && found) atomicOr(c.words, found);
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        if (atomicAdd(c.words + 1, 1u) == blocks - 1) {
-            const unsigned int all = atomicExch(c.words, 0u);
-            c.words[1] = 0;
-            fwd_publish(c, all);
-        }
+    const unsigned int all = (__syncthreads_or((int)(found & kFwdKeyRange)) ? kFwdKeyRange : 0u) |
+                             (__syncthreads_or((int)(found & kFwdValueRange)) ? kFwdValueRange : 0u);
+    if (threadIdx.x != 0) return;
+    unsigned int verdict = all;
+    if (blocks > 1) {
+        if (all) atomicOr(c.words, all);
+        __threadfence();
+        if (atomicAdd(c.words + 1, 1u) != blocks - 1) return;
+        verdict = atomicExch(c.words, 0u);
+        c.words[1] = 0;
     }
+    *(volatile unsigned long long*)c.status = ((unsigned long long)c.seq << 32) | verdict;
 }
 
 // Restores the caller's current device (the context's own may be another).
 struct FwdDevice {
-    int before = -1;
+    int before = -1, own;
     cudaError_t err;
-    explicit FwdDevice(const dpb_ctx* ctx) {
+    explicit FwdDevice(const dpb_ctx* ctx) : own(ctx->device) {
         err = cudaGetDevice(&before);
         if (err == cudaSuccess && before != ctx->device) err = cudaSetDevice(ctx->device);
     }
     ~FwdDevice() {
-        if (before >= 0) cudaSetDevice(before);
+        if (before >= 0 && before != own) cudaSetDevice(before);
     }
 };
 

@@ -23,109 +23,134 @@ struct LookupArgs {
 
 constexpr uint32_t kLookupThreads = 256;
 
-__device__ __forceinline__ int64_t lookup_scale(const LookupArgs& a, int64_t x) {
-    return (int64_t)((uint64_t)x * (uint64_t)a.multiplier + (uint64_t)a.rounding) >> a.shift;
+// the entry and the multiplier fit 32 bits, so that the product and the rounding fit 64
+__device__ __forceinline__ int64_t lookup_scale(const LookupArgs& a, int32_t x) {
+    return ((int64_t)x * (int32_t)a.multiplier + a.rounding) >> a.shift;
 }
-// whether x * m + r leaves 64 bits
-__device__ __forceinline__ bool lookup_overflows(const LookupArgs& a, int64_t x) {
+// any product; whether it leaves 64 bits goes to `over`
+__device__ __forceinline__ int64_t lookup_scale(const LookupArgs& a, int64_t x, bool& over) {
     const __int128 v = (__int128)x * a.multiplier + a.rounding;
-    return v != (__int128)(int64_t)v;
+    over = over || v != (__int128)(int64_t)v;
+    return (int64_t)v >> a.shift;
 }
 
-// T: the table's integers; V: entries per step (1 or 16 bytes' worth on the narrower side)
-template <class T, int V, bool CHECK>
-__global__ void __launch_bounds__(kLookupThreads) embedding_lookup_kernel(LookupArgs a) {
+// T: the table's integers; V: entries per step (1 or 16 bytes' worth on the narrower side).  I: the index type; 32 bits
+// wherever they suffice, since finding a step's row takes a division.  kLookupFlight steps per thread are under way
+// together: tokens, then table entries, then results.
+constexpr int kLookupFlight = 4;
+template <class T, int V, bool CHECK, class I>
+__global__ void __launch_bounds__(kLookupThreads, sizeof(I) == 4 ? 4 : 2) embedding_lookup_kernel(LookupArgs a) {
     unsigned int found = 0;
-    const uint64_t per_row = (a.out_width + V - 1) / V, total = a.out_rows * per_row;
-    const uint64_t step = (uint64_t)gridDim.x * kLookupThreads;
+    const bool small = a.multiplier == (int32_t)a.multiplier;
+    const I per_row = (I)((a.out_width + V - 1) / V), total = (I)a.out_rows * per_row;
+    const I step = (I)gridDim.x * kLookupThreads;
     if (!CHECK && blockIdx.x < a.check_blocks) {
         // the checking blocks look at all tokens first, so that the host need not wait for the rows
         for (uint64_t i = (uint64_t)blockIdx.x * kLookupThreads + threadIdx.x; i < a.n; i += (uint64_t)a.check_blocks * kLookupThreads)
             if ((uint64_t)a.tokens[i] >= a.vocab) found = kFwdKeyRange;
         fwd_check_done(a.check, found, a.check_blocks);
     }
-    for (uint64_t w = (uint64_t)blockIdx.x * kLookupThreads + threadIdx.x; w < total; w += step) {
-        const uint64_t i = w / per_row, c = (w - i * per_row) * V;
-        int64_t y[V];
+    for (I w0 = (I)blockIdx.x * kLookupThreads + threadIdx.x; w0 < total; w0 += kLookupFlight * step) {
+        uint64_t row[kLookupFlight], col[kLookupFlight], tok[kLookupFlight];
+        T x[kLookupFlight][V];
 #pragma unroll
-        for (int v = 0; v < V; v++) y[v] = 0;
-        if (i < a.n && c < a.width) {
-            const uint64_t t = (uint64_t)a.tokens[i];
-            if (t < a.vocab) {
-                const T* row = (const T*)a.table + t * a.stride + c;
-                T x[V];
-                if constexpr (V * sizeof(T) == 16) {
-                    *(int4*)x = __ldg((const int4*)row);
-                } else {
+        for (int f = 0; f < kLookupFlight; f++) {
+            const I w = w0 + f * step;  // 32 bits: total + kLookupFlight * step stays below 2^32 (the host's rule)
+            const I i = w / per_row;
+            row[f] = i;
+            col[f] = (uint64_t)(w - i * per_row) * V;
+            tok[f] = w < total && row[f] < a.n && col[f] < a.width ? (uint64_t)__ldg((const long long*)a.tokens + i) : ~0ull - 1;
+        }
 #pragma unroll
-                    for (int v = 0; v < V; v++) x[v] = __ldg(row + v);
-                }
+        for (int f = 0; f < kLookupFlight; f++) {
 #pragma unroll
-                for (int v = 0; v < V; v++) {
-                    if (V > 1 && c + v >= a.width) break;  // between the width and the stride
-                    y[v] = lookup_scale(a, (int64_t)x[v]);
-                    if (CHECK && lookup_overflows(a, (int64_t)x[v])) found |= kFwdValueRange;
-                }
-            } else if (CHECK) {
-                found |= kFwdKeyRange;
+            for (int v = 0; v < V; v++) x[f][v] = 0;
+            if (tok[f] < a.vocab) {
+                const T* src = (const T*)a.table + tok[f] * a.stride + col[f];
+                if constexpr (V * sizeof(T) == 16) *(int4*)x[f] = __ldg((const int4*)src);
+                else x[f][0] = __ldg(src);
             }
         }
-        int64_t* o = a.out + i * a.out_width + c;
-        if constexpr (V == 1) {
-            __stcs((long long*)o, (long long)y[0]);
-        } else {
 #pragma unroll
-            for (int v = 0; v < V; v += 2) __stcs((longlong2*)(o + v), make_longlong2(y[v], y[v + 1]));
+        for (int f = 0; f < kLookupFlight; f++) {
+            if (w0 + f * step >= total) break;
+            const bool live = tok[f] < a.vocab;
+            if (CHECK && !live && row[f] < a.n && col[f] < a.width) found |= kFwdKeyRange;
+            int64_t y[V];
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const bool in = live && (V == 1 || col[f] + v < a.width);  // not between the width and the stride
+                y[v] = 0;
+                if (!CHECK || (small && x[f][v] == (T)(int32_t)x[f][v])) {
+                    if (in) y[v] = lookup_scale(a, (int32_t)x[f][v]);
+                } else if (in) {
+                    bool over = false;
+                    y[v] = lookup_scale(a, (int64_t)x[f][v], over);
+                    if (over) found |= kFwdValueRange;
+                }
+            }
+            int64_t* o = a.out + row[f] * a.out_width + col[f];
+            if constexpr (V == 1) {
+                __stcs((long long*)o, (long long)y[0]);
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; v += 2) __stcs((longlong2*)(o + v), make_longlong2(y[v], y[v + 1]));
+            }
         }
     }
     if (CHECK) fwd_check_done(a.check, found, gridDim.x);
 }
 
 // ------------------------------------------------------------------------------------------------ rows by key
-// Up to kSmallSort rows: one block sorts (key, row) in shared memory by a bitonic network, one launch in all.
-constexpr uint32_t kSmallSort = 2048, kSmallSortThreads = 1024;
+// Up to kSmallSort rows: the place of a row is the number of rows that go before it (a smaller key, or the same key and
+// a smaller row), counted against all keys in shared memory by eight threads per row: n^2 comparisons over many SMs in
+// one launch, where a sorting network in one block waits at its barriers (2048 rows: 25 us) and a counting sort takes
+// three launches.  The first places of the keys, where they are kept, are counted the same way.
+constexpr uint32_t kSmallSort = 4096, kSmallSortThreads = 256;
 __global__ void __launch_bounds__(kSmallSortThreads)
-    groups_small_kernel(const int64_t* __restrict__ keys, uint32_t n, uint32_t n_keys, uint32_t n_pow2, uint32_t* __restrict__ out_keys,
-                        uint32_t* __restrict__ out_rows, uint32_t* __restrict__ offsets, FwdCheck check) {
-    __shared__ unsigned long long v[kSmallSort];
+    groups_small_kernel(const int64_t* __restrict__ keys, uint32_t n, uint32_t n_keys, uint32_t* __restrict__ out_keys,
+                        uint32_t* __restrict__ out_rows, uint32_t* __restrict__ places, uint32_t* __restrict__ offsets, FwdCheck check) {
+    extern __shared__ uint4 sh4[];
+    uint32_t* sh = (uint32_t*)sh4;
+    const uint32_t n_up = (n + 31) & ~31u;
     unsigned int found = 0;
-    for (uint32_t i = threadIdx.x; i < n_pow2; i += kSmallSortThreads) {
-        unsigned long long e = ~0ull;
+    for (uint32_t i = threadIdx.x; i < n_up; i += kSmallSortThreads) {
+        uint32_t k = 0xffffffffu;
         if (i < n) {
-            const uint64_t k = (uint64_t)keys[i];
-            if (k >= n_keys) found = kFwdKeyRange;
-            e = ((unsigned long long)(k < n_keys ? (uint32_t)k : n_keys) << 32) | i;
+            const uint64_t k64 = (uint64_t)keys[i];
+            if (k64 >= n_keys) found = kFwdKeyRange;
+            k = k64 < n_keys ? (uint32_t)k64 : n_keys;
         }
-        v[i] = e;
+        sh[i] = k;
     }
-    fwd_check_done(check, found, 1);
+    if (blockIdx.x == 0) fwd_check_done(check, found, 1);
     __syncthreads();
-    for (uint32_t size = 2; size <= n_pow2; size <<= 1)
-        for (uint32_t half = size >> 1; half > 0; half >>= 1) {
-            for (uint32_t p = threadIdx.x; p < n_pow2 / 2; p += kSmallSortThreads) {
-                const uint32_t i = 2 * p - (p & (half - 1)), j = i + half;
-                const unsigned long long x = v[i], y = v[j];
-                if ((x > y) == ((i & size) == 0)) {
-                    v[i] = y;
-                    v[j] = x;
-                }
-            }
-            __syncthreads();
+    const uint32_t t = blockIdx.x * kSmallSortThreads + threadIdx.x, part = t & 7, i = t >> 3;
+    const uint32_t probes = n + (offsets ? n_keys + 1 : 0);
+    const uint32_t k = i < n ? sh[i] : i - n;  // a row's key, or a key whose first place is asked for
+    uint32_t below = 0;
+    for (uint32_t q = part; q < n_up / 4; q += 8) {
+        const uint4 v = sh4[q];
+        // rows before i with the same key count as well: key <= k up to i, key < k from there on
+        const uint32_t j = 4 * q;
+        if (i < n && j + 4 <= i) {
+            below += (v.x <= k) + (v.y <= k) + (v.z <= k) + (v.w <= k);
+        } else {
+            below += (v.x < k) + (v.y < k) + (v.z < k) + (v.w < k);
+            if (i < n && j < i) below += (v.x == k) + (j + 1 < i && v.y == k) + (j + 2 < i && v.z == k);
         }
-    for (uint32_t i = threadIdx.x; i < n; i += kSmallSortThreads) {
-        out_keys[i] = (uint32_t)(v[i] >> 32);
-        out_rows[i] = (uint32_t)v[i];
     }
-    if (offsets)
-        for (uint32_t k = threadIdx.x; k <= n_keys; k += kSmallSortThreads) {
-            uint32_t lo = 0, hi = n;
-            while (lo < hi) {
-                const uint32_t mid = (lo + hi) >> 1;
-                if ((uint32_t)(v[mid] >> 32) < k) lo = mid + 1;
-                else hi = mid;
-            }
-            offsets[k] = lo;
+#pragma unroll
+    for (int off = 4; off > 0; off >>= 1) below += __shfl_down_sync(0xffffffffu, below, off);
+    if (part == 0 && i < probes) {
+        if (i < n) {
+            out_keys[below] = k;
+            out_rows[below] = i;
+            places[i] = below;
+        } else {
+            offsets[i - n] = below;
         }
+    }
 }
 
 // More rows: a counting sort.  rank[i] is the row's place inside its key; equal keys of a warp share one atomic.
@@ -192,7 +217,7 @@ __global__ void __launch_bounds__(1024)
 // tiles <= 1025: every block adds the tiles' sums up for itself
 __global__ void __launch_bounds__(kThreads)
     groups_scatter_kernel(const int64_t* __restrict__ keys, uint32_t n, uint32_t n_keys, const uint32_t* __restrict__ counts,
-                          const uint32_t* __restrict__ tile_sums, uint32_t tiles, const uint32_t* __restrict__ rank,
+                          const uint32_t* __restrict__ tile_sums, uint32_t tiles, uint32_t* __restrict__ rank,
                           uint32_t* __restrict__ out_keys, uint32_t* __restrict__ out_rows) {
     __shared__ uint32_t before[1056];
     if (threadIdx.x < 32) {
@@ -217,6 +242,7 @@ __global__ void __launch_bounds__(kThreads)
         const uint32_t p = before[k / kCountTile] + counts[k] + rank[i];
         out_keys[p] = k;
         out_rows[p] = (uint32_t)i;
+        rank[i] = p;  // from here on the row's place in the whole order
     }
 }
 
@@ -239,33 +265,53 @@ struct RowSumArgs {
     void* parts;  // [slice][2][width]
 };
 
-// An unreduced sum of (weight) * (integer) products, or of plain integers.
+// An unreduced sum of (weight) * (integer) products, or of plain integers.  Entries that fit 32 bits, as quantised
+// values do, enter as x + 2^31, an unsigned word: a product is then 8 wide multiply-adds for BN254 (4 for the two words
+// of each Goldilocks component) with no sign to look at, and the sum is 2^31 times the sum of the weights too large,
+// which `shift_back` takes back when the key's run ends.  Wider entries enter by magnitude with the weight or its
+// negative, plus 2^31 times the weight so that the same correction applies.
 template <class F, bool W>
 struct RowAccum;
 template <>
 struct RowAccum<FrFam, true> {
-    FrIntAcc s;
-    __device__ __forceinline__ void zero() { s = fr_intacc_zero(); }
-    // w: the weight and its negative, 8 words each
-    __device__ __forceinline__ void mac(const Fr* w, int64_t x) {
-        const uint64_t mag = x < 0 ? (uint64_t)0 - (uint64_t)x : (uint64_t)x;
-        frw::intacc_mac(s.a, frw::from_fr(w[x < 0]), mag);
+    frw::RowAcc s;  // below 2^286 per term: the words above 7 count carries only, so their 32 bits hold any run
+    __device__ __forceinline__ void zero() { s = frw::rowacc_zero(); }
+    __device__ __forceinline__ void mac32(const frw::F8& w, int32_t x) { frw::rowacc_mac(s, w.w, (uint32_t)x ^ 0x80000000u); }
+    static __device__ __forceinline__ frw::F8 weight(const Fr& w) { return frw::from_fr(w); }
+    // the sum, `more` added, as a field element; wsum = the sum of the weights
+    __device__ __forceinline__ Fr finish(const Fr& wsum, const Fr& more) const {
+        FrIntAcc t;
+#pragma unroll
+        for (int i = 0; i < 12; i++) {
+            t.a.E[i] = i <= 8 ? s.E[i] : 0;
+            t.a.O[i] = i <= 9 ? s.O[i] : 0;
+        }
+        frw::intacc_mac_lo(t.a, frw::from_fr(fr_neg(wsum)), 0x80000000u);
+        return fr_add(fr_intacc_finish(t), more);
     }
-    __device__ __forceinline__ Fr finish() const { return fr_intacc_finish(s); }
 };
 template <>
 struct RowAccum<GlFam, true> {
     glw::A8 s0, s1;
     __device__ __forceinline__ void zero() { s0 = s1 = glw::acc_zero(); }
-    __device__ __forceinline__ void mac(const Gl2* w, int64_t x) {
-        const uint64_t mag = x < 0 ? (uint64_t)0 - (uint64_t)x : (uint64_t)x;
-        const glw::W2 ww = gl2_words(w[x < 0]);
-        const glw::W m = glw::make_w((uint32_t)mag, (uint32_t)(mag >> 32));
-        glw::acc_mac(s0, m, ww.c0);
-        glw::acc_mac(s1, m, ww.c1);
+    static __device__ __forceinline__ void mac(glw::A8& s, const glw::W& w, uint32_t u) {
+        asm("mad.lo.cc.u32 %0, %6, %8, %0; madc.hi.cc.u32 %1, %6, %8, %1; addc.u32 %2, %2, 0;\n\t"
+            "mad.lo.cc.u32 %3, %7, %8, %3; madc.hi.cc.u32 %4, %7, %8, %4; addc.u32 %5, %5, 0;"
+            : "+r"(s.e0), "+r"(s.e1), "+r"(s.e2), "+r"(s.o1), "+r"(s.o2), "+r"(s.o3)
+            : "r"(w.lo), "r"(w.hi), "r"(u));
     }
-    __device__ __forceinline__ Gl2 finish() const {
-        return gl2_make(glw::to_u64(glw::canon(glw::acc_reduce(s0))), glw::to_u64(glw::canon(glw::acc_reduce(s1))));
+    __device__ __forceinline__ void mac32(const glw::W2& w, int32_t x) {
+        mac(s0, w.c0, (uint32_t)x ^ 0x80000000u);
+        mac(s1, w.c1, (uint32_t)x ^ 0x80000000u);
+    }
+    static __device__ __forceinline__ glw::W2 weight(const Gl2& w) { return gl2_words(w); }
+    __device__ __forceinline__ Gl2 finish(const Gl2& wsum, const Gl2& more) const {
+        glw::A8 t0 = s0, t1 = s1;
+        const glw::W2 n = gl2_words(gl2_neg(wsum));
+        // one more term; the words next to e1 and o2 count carries only, and no run has 2^32 terms
+        mac(t0, n.c0, 0x80000000u);
+        mac(t1, n.c1, 0x80000000u);
+        return GlFam::add(gl2_make(glw::to_u64(glw::canon(glw::acc_reduce(t0))), glw::to_u64(glw::canon(glw::acc_reduce(t1)))), more);
     }
 };
 template <class F>
@@ -276,29 +322,46 @@ __device__ __forceinline__ typename F::E field_from_i128(__int128 v) {
     if ((uint64_t)(m >> 64)) r = F::add(r, F::mul(F::from_u64((uint64_t)(m >> 64)), F::from_u64_pow64()));
     return neg ? F::neg(r) : r;
 }
-template <class F>
-struct RowAccum<F, false> {
-    __int128 s;
-    __device__ __forceinline__ void zero() { s = 0; }
-    __device__ __forceinline__ void mac(const typename F::E*, int64_t x) { s += x; }
-    __device__ __forceinline__ typename F::E finish() const { return field_from_i128<F>(s); }
-};
 
+// v += w * (x - its low 32 bits as a signed word), for the rare entry that has more than those
+template <class F>
+__device__ __noinline__ typename F::E add_high(typename F::E v, const typename F::E w, int64_t x) {
+    const int64_t hi = (x >> 32) + ((int32_t)x < 0 ? 1 : 0);
+    if (hi == 0) return v;
+    const typename F::E t = F::mul(w, F::mul(F::from_u64(hi < 0 ? (uint64_t)0 - (uint64_t)hi : (uint64_t)hi), F::from_u64(1ull << 32)));
+    return hi < 0 ? F::sub(v, t) : F::add(v, t);
+}
+
+// A block: neighbouring columns of one slice.  Rows come in batches whose weights, and the weights'
+// prefix sums, go through shared memory; kRowSumFlight rows' entries are loaded ahead of the products.
 constexpr uint32_t kRowSumThreads = 128, kRowSumBatch = 64, kRowSumFlight = 8;
 
-template <class F, bool W>
+// two neighbouring columns per thread with weights (a weight read from shared memory then serves two products)
+template <class F>
 __global__ void __launch_bounds__(kRowSumThreads)
-    row_sums_kernel(RowSumArgs a, typename F::E multiplier, bool scale) {
+    row_products_kernel(RowSumArgs a, typename F::E multiplier, bool scale) {
     typedef typename F::E E;
-    __shared__ E wsh[W ? kRowSumBatch : 1][2];
+    constexpr int C = 2;
+    __shared__ E wsh[kRowSumBatch], prefix[kRowSumBatch];
     __shared__ uint64_t at[kRowSumBatch];
-    __shared__ uint32_t ends[kRowSumBatch];  // key + 1 where the key's run ends here, else 0
-    const uint64_t c = (uint64_t)blockIdx.x * kRowSumThreads + threadIdx.x;
+    __shared__ uint32_t keys[kRowSumBatch];
+    __shared__ uint32_t ends[kRowSumBatch / 32];  // a bit per row: the key's run ends here
+    const uint64_t c0 = (uint64_t)blockIdx.x * (kRowSumThreads * C) + threadIdx.x;
     const uint64_t begin = blockIdx.y * a.slice, end = begin + a.slice < a.n ? begin + a.slice : a.n;
-    const bool live = c < a.width;
+    const uint32_t lane = threadIdx.x & 31;
+    bool live[C];
+#pragma unroll
+    for (int q = 0; q < C; q++) live[q] = c0 + q * kRowSumThreads < a.width;
     bool before = begin > 0 && a.keys[begin - 1] == a.keys[begin];  // the current run began before the slice
-    RowAccum<F, W> acc;
-    acc.zero();
+    RowAccum<F, true> acc[C];
+    E wide[C];  // what the entries of more than 32 bits add (seldom any)
+    bool any_wide = false;
+#pragma unroll
+    for (int q = 0; q < C; q++) {
+        acc[q].zero();
+        wide[q] = F::zero();
+    }
+    E run_weights = F::zero();  // of the run's rows in earlier batches
     for (uint64_t p0 = begin; p0 < end; p0 += kRowSumBatch) {
         const uint32_t m = end - p0 < kRowSumBatch ? (uint32_t)(end - p0) : kRowSumBatch;
         __syncthreads();
@@ -307,41 +370,163 @@ __global__ void __launch_bounds__(kRowSumThreads)
             const uint64_t p = p0 + i;
             const uint32_t row = a.rows[p], key = a.keys[p];
             at[threadIdx.x] = (uint64_t)(row / a.per) * a.width;
-            ends[threadIdx.x] = threadIdx.x < m && (p + 1 == end || a.keys[p + 1] != key) ? key + 1 : 0;
-            if (W) {
-                const E w = F::load(a.weights, F::kChalDtype, row);
-                wsh[threadIdx.x][0] = w;
-                wsh[threadIdx.x][1] = F::neg(w);
+            keys[threadIdx.x] = key;
+            const uint32_t run_ends = __ballot_sync(0xffffffffu, threadIdx.x < m && (p + 1 == end || a.keys[p + 1] != key));
+            if (lane == 0) ends[threadIdx.x >> 5] = run_ends;
+            const E w = F::load(a.weights, F::kChalDtype, row);
+            wsh[threadIdx.x] = w;
+            E sum = w;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const E o = F::shfl_up(sum, off);
+                if (lane >= (uint32_t)off) sum = F::add(sum, o);
             }
+            prefix[threadIdx.x] = sum;
         }
         __syncthreads();
-        for (uint32_t i0 = 0; i0 < m; i0 += kRowSumFlight) {
-            int64_t x[kRowSumFlight];
+        // the weights of rows s..i of the batch: the prefix sums run inside each half of 32
+        auto weights_of = [&](uint32_t s, uint32_t i) {
+            E v = prefix[i];
+            if (s < 32 && i >= 32) v = F::add(v, prefix[31]);
+            if (s & 31) v = F::sub(v, prefix[s - 1]);
+            return v;
+        };
+        // one run, or the part of it in this batch, after the other; the loop over its rows holds the products alone, so
+        // that it stays in the instruction cache (with the ends of runs unrolled into it: 158 us instead of 37)
+        const uint64_t run_ends = ends[0] | (uint64_t)ends[1] << 32;
+        for (uint32_t s = 0; s < m;) {
+            const uint64_t rest = run_ends >> s;
+            const uint32_t t = rest ? s + __ffsll(rest) - 1 : m - 1;  // the run's last row here
+            for (uint32_t i0 = s; i0 <= t; i0 += kRowSumFlight) {
+                int64_t x[kRowSumFlight][C];
+                int64_t high = 0;
 #pragma unroll
-            for (uint32_t u = 0; u < kRowSumFlight; u++) x[u] = live && i0 + u < m ? __ldg(a.x + at[i0 + u] + c) : 0;
+                for (uint32_t u = 0; u < kRowSumFlight; u++)
 #pragma unroll
-            for (uint32_t u = 0; u < kRowSumFlight; u++) {
-                if (i0 + u >= m) break;
-                acc.mac(wsh[W ? i0 + u : 0], x[u]);
-                if (ends[i0 + u]) {
-                    const uint32_t key = ends[i0 + u] - 1;
-                    const uint64_t p = p0 + i0 + u;
-                    const bool after = p + 1 == end && end < a.n && a.keys[end] == key;
-                    if (live) {
-                        E v = acc.finish();
+                    for (int q = 0; q < C; q++)
+                        x[u][q] = live[q] && i0 + u <= t ? __ldg((const long long*)a.x + at[i0 + u] + c0 + q * kRowSumThreads) : 0;
+#pragma unroll
+                for (uint32_t u = 0; u < kRowSumFlight; u++) {
+                    if (i0 + u > t) break;
+                    const auto w = RowAccum<F, true>::weight(wsh[i0 + u]);
+#pragma unroll
+                    for (int q = 0; q < C; q++) {
+                        acc[q].mac32(w, (int32_t)x[u][q]);
+                        high |= x[u][q] - (int32_t)x[u][q];
+                    }
+                }
+                if (high) {
+                    any_wide = true;
+#pragma unroll 1
+                    for (uint32_t u = 0; u < kRowSumFlight && i0 + u <= t; u++)
+#pragma unroll
+                        for (int q = 0; q < C; q++)
+                            if (live[q]) wide[q] = add_high<F>(wide[q], wsh[i0 + u], a.x[at[i0 + u] + c0 + q * kRowSumThreads]);
+                }
+            }
+            const E ws = weights_of(s, t);
+            if (rest) {
+                const uint32_t key = keys[t];
+                const bool after = p0 + t + 1 == end && end < a.n && a.keys[end] == key;
+                const E total = F::add(run_weights, ws);
+#pragma unroll
+                for (int q = 0; q < C; q++) {
+                    if (live[q]) {
+                        const uint64_t c = c0 + q * kRowSumThreads;
+                        E v = acc[q].finish(total, wide[q]);
                         if (before || after) {
-                            F::store(a.parts, (blockIdx.y * 2 + (before ? 0 : 1)) * a.width + c, v);
+                            F::store(a.parts, ((uint64_t)blockIdx.y * 2 + (before ? 0 : 1)) * a.width + c, v);
                         } else {
                             if (scale) v = F::mul(v, multiplier);
                             F::store(a.out, (uint64_t)key * a.out_width + c, v);
                         }
                     }
-                    acc.zero();
+                }
+#pragma unroll
+                for (int q = 0; q < C; q++) {
+                    acc[q].zero();
+                    if (any_wide) wide[q] = F::zero();
+                }
+                any_wide = false;
+                before = false;
+                run_weights = F::zero();
+            } else {
+                run_weights = F::add(run_weights, ws);
+            }
+            s = t + 1;
+        }
+    }
+}
+
+template <class F>
+__device__ __noinline__ void store_sum(__int128 sum, bool part, bool scale, const typename F::E& multiplier, void* out, uint64_t i) {
+    typename F::E v = field_from_i128<F>(sum);
+    if (scale && !part) v = F::mul(v, multiplier);
+    F::store(out, i, v);
+}
+
+// the integers alone: 128-bit sums, one column per thread
+template <class F>
+__global__ void __launch_bounds__(kRowSumThreads)
+    row_sums_kernel(RowSumArgs a, typename F::E multiplier, bool scale) {
+    typedef typename F::E E;
+    __shared__ uint64_t at[kRowSumBatch];
+    __shared__ uint32_t ends[kRowSumBatch];
+    const uint64_t c = (uint64_t)blockIdx.x * kRowSumThreads + threadIdx.x;
+    const uint64_t begin = blockIdx.y * a.slice, end = begin + a.slice < a.n ? begin + a.slice : a.n;
+    const bool live = c < a.width;
+    bool before = begin > 0 && a.keys[begin - 1] == a.keys[begin];
+    __int128 acc = 0;
+    for (uint64_t p0 = begin; p0 < end; p0 += kRowSumBatch) {
+        const uint32_t m = end - p0 < kRowSumBatch ? (uint32_t)(end - p0) : kRowSumBatch;
+        __syncthreads();
+        if (threadIdx.x < kRowSumBatch) {
+            const uint64_t p = p0 + (threadIdx.x < m ? threadIdx.x : m - 1);
+            const uint32_t key = a.keys[p];
+            at[threadIdx.x] = (uint64_t)(a.rows[p] / a.per) * a.width;
+            ends[threadIdx.x] = threadIdx.x < m && (p + 1 == end || a.keys[p + 1] != key) ? key + 1 : 0;
+        }
+        __syncthreads();
+        for (uint32_t i0 = 0; i0 < m; i0 += kRowSumFlight) {
+            int64_t x[kRowSumFlight];
+#pragma unroll
+            for (uint32_t u = 0; u < kRowSumFlight; u++)
+                x[u] = live && i0 + u < m ? __ldg((const long long*)a.x + at[i0 + u] + c) : 0;
+#pragma unroll
+            for (uint32_t u = 0; u < kRowSumFlight; u++) {
+                const uint32_t i = i0 + u;
+                if (i >= m) break;
+                acc += x[u];
+                if (ends[i]) {
+                    const uint32_t key = ends[i] - 1;
+                    const bool after = p0 + i + 1 == end && end < a.n && a.keys[end] == key;
+                    if (live) {
+                        const uint64_t slot = ((uint64_t)blockIdx.y * 2 + (before ? 0 : 1)) * a.width + c;
+                        store_sum<F>(acc, before || after, scale, multiplier, before || after ? a.parts : a.out,
+                                     before || after ? slot : (uint64_t)key * a.out_width + c);
+                    }
+                    acc = 0;
                     before = false;
                 }
             }
         }
     }
+}
+
+// First place whose key is not below `key`, by a warp: 32 probes per step.
+__device__ __forceinline__ uint64_t warp_first_at(const uint32_t* __restrict__ keys, uint64_t n, uint64_t key) {
+    uint64_t lo = 0, hi = n;  // the answer lies in [lo, hi]
+    const uint32_t lane = threadIdx.x & 31;
+    while (lo < hi) {
+        const uint64_t step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const bool below = at < hi && keys[at] < key;
+        const uint32_t k = __popc(__ballot_sync(0xffffffffu, below));  // probes 0..k-1 are below
+        if (k == 0) return lo;
+        const uint64_t next = lo + k * step;
+        lo = lo + (uint64_t)(k - 1) * step + 1;
+        if (next < hi) hi = next;
+    }
+    return lo;
 }
 
 // Adds up the keys that span slices: block row y looks at slice y, and acts when a key begins there and goes on.
@@ -352,26 +537,32 @@ __global__ void __launch_bounds__(kRowSumThreads)
     const uint64_t begin = blockIdx.y * a.slice, end = begin + a.slice;
     if (end >= a.n) return;
     const uint32_t key = a.keys[end - 1];
-    if (a.keys[end] != key) return;                                                // nothing goes on
-    if (begin > 0 && a.keys[begin - 1] == key) return;                             // it began before
+    if (a.keys[end] != key) return;                     // nothing goes on
+    if (begin > 0 && a.keys[begin - 1] == key) return;  // it began before
+    const uint64_t last = (warp_first_at(a.keys, a.n, (uint64_t)key + 1) - 1) / a.slice;
     const uint64_t c = (uint64_t)blockIdx.x * kRowSumThreads + threadIdx.x;
     if (c >= a.width) return;
-    E v = F::load(a.parts, F::kChalDtype, (blockIdx.y * 2 + 1) * a.width + c);
-    for (uint64_t s = blockIdx.y + 1; s * a.slice < a.n && a.keys[s * a.slice] == key; s++)
-        v = F::add(v, F::load(a.parts, F::kChalDtype, (s * 2) * a.width + c));
+    E v = F::load(a.parts, F::kChalDtype, ((uint64_t)blockIdx.y * 2 + 1) * a.width + c);
+    for (uint64_t s = blockIdx.y + 1; s <= last; s += 4) {
+        E part[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) part[u] = s + u <= last ? F::load(a.parts, F::kChalDtype, ((s + u) * 2) * a.width + c) : F::zero();
+#pragma unroll
+        for (int u = 0; u < 4; u++) v = F::add(v, part[u]);
+    }
     if (scale) v = F::mul(v, multiplier);
     F::store(a.out, (uint64_t)key * a.out_width + c, v);
 }
 
 // Sums of the weights alone (one column).  Two kinds of blocks in one launch: the first `key_blocks` own 256 keys each,
 // a thread per key, which adds the key's rows when they are few and writes the table's zeros; the others own a slice of
-// the sorted order and add up, with all their threads, the keys that have many.
-constexpr uint32_t kKeySumThreads = 256, kKeySumFew = 16;
+// the sorted order, and their warps add up the keys that have many.
+constexpr uint32_t kKeySumThreads = 256, kKeySumFew = 8, kKeySumSlice = 512;
 template <class F, bool W>
 __global__ void __launch_bounds__(kKeySumThreads)
     key_sums_kernel(RowSumArgs a, uint64_t n_keys, uint64_t out_keys, uint32_t key_blocks, typename F::E multiplier, bool scale) {
     typedef typename F::E E;
-    const uint32_t tid = threadIdx.x;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto first_at = [&](uint64_t lo, uint64_t hi, uint64_t key) {  // first place in [lo, hi) whose key is not below
         while (lo < hi) {
             const uint64_t mid = (lo + hi) >> 1;
@@ -383,26 +574,43 @@ __global__ void __launch_bounds__(kKeySumThreads)
     if (blockIdx.x < key_blocks) {
         __shared__ uint64_t range[2];
         const uint64_t k0 = (uint64_t)blockIdx.x * kKeySumThreads, k = k0 + tid;
-        if (tid < 2) range[tid] = first_at(0, a.n, k0 + tid * kKeySumThreads);
+        if (warp < 2) {
+            const uint64_t p = warp_first_at(a.keys, a.n, k0 + warp * kKeySumThreads);
+            if (lane == 0) range[warp] = p;
+        }
         __syncthreads();
         if (k >= out_keys) return;
         E v = F::zero();
         if (k < n_keys && range[0] < range[1]) {
-            const uint64_t lo = first_at(range[0], range[1], k), hi = first_at(lo, range[1], k + 1);
-            if (hi - lo > kKeySumFew) return;  // the slices' blocks write it
-            if (W) {
-                for (uint64_t p = lo; p < hi; p++) v = F::add(v, F::load(a.weights, F::kChalDtype, a.rows[p]));
-            } else {
-                v = F::from_u64(hi - lo);
+            const uint64_t lo = first_at(range[0], range[1], k);
+            uint32_t count = 0;
+            uint32_t row[kKeySumFew];
+            bool mine = lo < range[1];
+#pragma unroll
+            for (uint32_t j = 0; j < kKeySumFew; j++) {
+                mine = mine && lo + j < range[1] && a.keys[lo + j] == k;
+                row[j] = mine ? a.rows[lo + j] : 0xffffffffu;
+                count += mine;
             }
-            if (scale) v = F::mul(v, multiplier);
+            if (mine && lo + kKeySumFew < range[1] && a.keys[lo + kKeySumFew] == k) return;  // the slices' blocks write it
+            if (W) {
+                E w[kKeySumFew];  // all loads under way before the first sum
+#pragma unroll
+                for (uint32_t j = 0; j < kKeySumFew; j++) w[j] = row[j] != 0xffffffffu ? F::load(a.weights, F::kChalDtype, row[j]) : F::zero();
+#pragma unroll
+                for (uint32_t j = 0; j < kKeySumFew; j++)
+                    if (j < count) v = F::add(v, w[j]);
+            } else {
+                v = F::from_u64(count);
+            }
+            if (scale && count) v = F::mul(v, multiplier);
         }
         F::store(a.out, k, v);
         return;
     }
     const uint64_t s = blockIdx.x - key_blocks, begin = s * a.slice, end = begin + a.slice < a.n ? begin + a.slice : a.n;
     __shared__ uint32_t n_long;
-    __shared__ uint64_t starts[64];  // runs of more than kKeySumFew rows that touch the slice: at most slice / 16 + 2
+    __shared__ uint32_t starts[kKeySumSlice / (kKeySumFew + 1) + 2];  // runs of more than kKeySumFew rows in the slice
     if (tid == 0) n_long = 0;
     __syncthreads();
     for (uint64_t p = begin + tid; p < end; p += kKeySumThreads) {
@@ -410,27 +618,46 @@ __global__ void __launch_bounds__(kKeySumThreads)
         if (p > begin && a.keys[p - 1] == key) continue;  // not where a run enters the slice
         bool is_long = p + kKeySumFew < a.n && a.keys[p + kKeySumFew] == key;
         if (!is_long && p == begin && begin > 0 && a.keys[begin - 1] == key) {
-            const uint64_t lo = first_at(0, begin, key), hi = first_at(begin, a.n, (uint64_t)key + 1);
+            // the tail of a run that entered before: its length decides
+            uint64_t hi = p + 1, lo = p;
+            while (hi < a.n && a.keys[hi] == key) hi++;                                  // at most kKeySumFew steps
+            while (lo > 0 && hi - lo <= kKeySumFew && a.keys[lo - 1] == key) lo--;
             is_long = hi - lo > kKeySumFew;
         }
-        if (is_long) starts[atomicAdd(&n_long, 1u)] = p;
+        if (is_long) starts[atomicAdd(&n_long, 1u)] = (uint32_t)(p - begin);
     }
     __syncthreads();
     const uint32_t count = n_long;
-    for (uint32_t r = 0; r < count; r++) {
-        const uint64_t p = starts[r];
+    for (uint32_t r = warp; r < count; r += kKeySumThreads / 32) {
+        const uint64_t p = begin + starts[r];
         const uint32_t key = a.keys[p];
-        uint64_t hi = end;
-        if (a.keys[end - 1] != key) hi = first_at(p, end, (uint64_t)key + 1);
-        E acc[1] = {F::zero()};
-        if (W) {
-            for (uint64_t q = p + tid; q < hi; q += kKeySumThreads) acc[0] = F::add(acc[0], F::load(a.weights, F::kChalDtype, a.rows[q]));
-            block_sum<F, 1>(acc);
+        E v = F::zero();
+        uint64_t rows = 0;
+        for (uint64_t q0 = p; q0 < end; q0 += 128) {
+            bool in[4];
+            E w[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint64_t q = q0 + 32 * j + lane;
+                in[j] = q < end && a.keys[q] == key;
+                if (W) w[j] = in[j] ? F::load(a.weights, F::kChalDtype, a.rows[q]) : F::zero();
+                rows += __popc(__ballot_sync(0xffffffffu, in[j]));
+            }
+            if (W) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) v = F::add(v, w[j]);
+            }
+            if (!__shfl_sync(0xffffffffu, (int)in[3], 31)) break;  // the run ended
         }
-        if (tid == 0) {
-            E v = W ? acc[0] : F::from_u64(hi - p);
+        if (W) {
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) v = F::add(v, F::shfl_down(v, off));
+        } else {
+            v = F::from_u64(rows);
+        }
+        if (lane == 0) {
             const bool before = p == begin && begin > 0 && a.keys[begin - 1] == key;
-            const bool after = hi == end && end < a.n && a.keys[end] == key;
+            const bool after = p + rows == end && end < a.n && a.keys[end] == key;
             if (before || after) {
                 F::store(a.parts, s * 2 + (before ? 0 : 1), v);
             } else {
@@ -438,7 +665,6 @@ __global__ void __launch_bounds__(kKeySumThreads)
                 F::store(a.out, key, v);
             }
         }
-        __syncthreads();
     }
 }
 

@@ -105,41 +105,52 @@ __device__ __forceinline__ void expert_tiles(const uint32_t* __restrict__ offset
     }
 }
 
-// Routed rows in sorted order -> planes [row tile][128 of the inner dimension][digit][T rows x 128 bytes].  A thread cuts
-// 16 entries of a row.  Rows of a tile past the expert's last are left as they are: their products are not stored.
+// Routed rows in sorted order -> planes [row tile][128 of the inner dimension][digit][T rows x 128 bytes].  A warp cuts
+// 256 entries of a row: it reads them as whole lines, whatever their alignment, and turns the digits round in shared
+// memory so that a lane writes 16 bytes.  Rows of a tile past the expert's last are left as they are: their products are
+// not stored.
+constexpr uint32_t kCutEntries = 256;
 template <int DIGITS>
 __global__ void __launch_bounds__(kCutThreads)
-    cut_rows_kernel(const int64_t* __restrict__ x, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ rows,
-                    const uint32_t* __restrict__ offsets, uint64_t n, uint32_t per, uint32_t n_experts, uint64_t inner,
+    cut_rows_kernel(const int64_t* __restrict__ x, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ places,
+                    const uint32_t* __restrict__ offsets, uint64_t tokens, uint32_t per, uint32_t n_experts, uint64_t inner,
                     uint32_t k_blocks, uint32_t rows_log2, int64_t half, int8_t* __restrict__ planes, FwdCheck check) {
     extern __shared__ uint32_t tiles[];
+    __shared__ __align__(16) uint8_t cut[kCutThreads / 32][DIGITS][kCutEntries];
     unsigned int found = 0;
     expert_tiles(offsets, n_experts, rows_log2, tiles);
     __syncthreads();
-    const uint32_t pieces = k_blocks * 8, T = 1u << rows_log2;
-    const uint64_t total = n * pieces;
-    const bool aligned = (inner & 1) == 0 && ((uintptr_t)x & 15) == 0;
-    for (uint64_t t = (uint64_t)blockIdx.x * kCutThreads + threadIdx.x; t < total; t += (uint64_t)gridDim.x * kCutThreads) {
-        const uint64_t p = t / pieces;
-        const uint32_t piece = (uint32_t)(t - p * pieces), e = keys[p];
-        if (e >= n_experts) continue;
-        const int64_t* src = x + (uint64_t)(rows[p] / per) * inner + piece * 16;
-        const uint64_t left = inner > piece * 16 ? inner - piece * 16 : 0;
-        int64_t v[16];
-        if (aligned && left >= 16) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, T = 1u << rows_log2;
+    const uint32_t per_row = (k_blocks + 1) / 2;  // 256 entries = two stages
+    const uint64_t total = tokens * per_row, step = (uint64_t)gridDim.x * (kCutThreads / 32);
+    for (uint64_t t = (uint64_t)blockIdx.x * (kCutThreads / 32) + warp; t < total; t += step) {
+        const uint64_t token = t / per_row;
+        const uint32_t k0 = (uint32_t)(t - token * per_row) * kCutEntries;
+        const int64_t* src = x + token * inner;
+        int64_t v[kCutEntries / 32];
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) *(longlong2*)(v + i) = __ldg((const longlong2*)(src + i));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; i++) v[i] = i < left ? __ldg(src + i) : 0;
+        for (uint32_t i = 0; i < kCutEntries / 32; i++) {
+            const uint64_t k = k0 + 32 * i + lane;
+            v[i] = k < inner ? __ldg((const long long*)src + k) : 0;
         }
-        uint4 d[DIGITS];
-        if (!cut_digits<DIGITS>(v, half, d)) found = kFwdValueRange;
-        const uint32_t at = (uint32_t)p - offsets[e];
-        const uint64_t tile = (uint64_t)(tiles[e] + (at >> rows_log2)) * k_blocks + piece / 8;
 #pragma unroll
-        for (int i = 0; i < DIGITS; i++)
-            *(uint4*)(planes + (tile * DIGITS + i) * (T * 128) + tile_piece(at & (T - 1), piece & 7)) = d[i];
+        for (uint32_t i = 0; i < kCutEntries / 32; i++) {
+            if (v[i] < -half || v[i] >= half) found = kFwdValueRange;
+            const int lo = (int)(int8_t)v[i];
+            cut[warp][0][32 * i + lane] = (uint8_t)lo;
+            if (DIGITS == 2) cut[warp][DIGITS - 1][32 * i + lane] = (uint8_t)(((int)v[i] - lo) >> 8);
+        }
+        __syncwarp();
+        const uint32_t piece = lane & 15, digit = lane >> 4, block = k0 / kTileK + piece / 8;
+        if (digit < DIGITS && block < k_blocks) {
+            const uint4 bytes = *(const uint4*)&cut[warp][digit][16 * piece];
+            for (uint32_t j = 0; j < per; j++) {
+                const uint32_t p = places[token * per + j], e = keys[p], at = p - offsets[e];
+                const uint64_t tile = (uint64_t)(tiles[e] + (at >> rows_log2)) * k_blocks + block;
+                *(uint4*)(planes + (tile * DIGITS + digit) * (T * 128) + tile_piece(at & (T - 1), piece & 7)) = bytes;
+            }
+        }
+        __syncwarp();
     }
     fwd_check_done(check, found, gridDim.x);
 }

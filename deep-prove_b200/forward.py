@@ -2,6 +2,7 @@
 transposes.  Device tensors are (table, shape) pairs, as Context.upload_tensor_i64 returns them; results of that form can
 be handed to the einsum and lookup calls' device_tensor arguments."""
 import ctypes
+import math
 
 import numpy as np
 
@@ -28,7 +29,7 @@ def _source(array, device):
     """(pointer, 1 when on the device, shape, what must stay alive) of an int64 tensor given either way."""
     if device is not None:
         mle, shape = device
-        return ctypes.c_void_p(lib.dpb_mle_device_ptr(mle.h)), 1, tuple(shape), mle
+        return lib.dpb_mle_device_ptr(mle.h), 1, shape, mle
     a = np.ascontiguousarray(array, dtype=np.int64)
     return _buf(a), 0, a.shape, a
 
@@ -43,7 +44,7 @@ def embedding_lookup(ctx, table, vocab, width, tokens, multiplier=1, right_shift
     (default: width) entries apart.  Returns (table, shape): the [n, width] tensor, or with padded=True the table of
     the padded shape."""
     ptr, on_device, shape, _keep = _source(tokens, device_tokens)
-    n = int(np.prod(shape, dtype=np.int64))
+    n = math.prod(shape)
     h = ctypes.c_void_p()
     check(lib.dpb_embedding_lookup(ctx.h, table.h, vocab, width, width if row_stride is None else row_stride, ptr, on_device, n,
                                    multiplier, right_shift, 1 if padded else 0, ctypes.byref(h)))
@@ -56,7 +57,7 @@ class RowGroups:
     def __init__(self, ctx, keys, n_keys, device_keys=None):
         self.ctx, self.h = ctx, None
         ptr, on_device, shape, _keep = _source(keys, device_keys)
-        self.n, self.n_keys = int(np.prod(shape, dtype=np.int64)), int(n_keys)
+        self.n, self.n_keys = math.prod(shape), int(n_keys)
         h = ctypes.c_void_p()
         check(lib.dpb_row_groups_new(ctx.h, ptr, on_device, self.n, n_keys, ctypes.byref(h)))
         self.h = h
