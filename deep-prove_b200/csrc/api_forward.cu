@@ -255,8 +255,13 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
     } else {
         rc = fwd_tensor(ctx, rows, rows_on_device, (a.n + per - 1) / per * width, &a.x, &owned);
         const uint64_t per_block = weights ? 2 * kRowSumThreads : kRowSumThreads, col_blocks = (width + per_block - 1) / per_block;
-        // slices of at least 16 rows, and no more of them than fill the GPU some times over
-        const uint64_t want = std::min<uint64_t>(65535, std::max<uint64_t>(1, (uint64_t)ctx->sm_count * 8 / col_blocks));
+        // slices of at least 16 rows, and as many as make one wave of resident blocks: the reduction at the end of a
+        // block's sums, some hundred rows' worth of products, is then paid the fewest times
+        int resident = 1;
+        const cudaError_t oe = weights ? cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, row_products_kernel<F, true>, kRowSumThreads, 0)
+                                       : cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, row_sums_kernel<F>, kRowSumThreads, 0);
+        if (rc == DPB_OK && oe != cudaSuccess) rc = fail(DPB_ECUDA, "row sums: %s", cudaGetErrorString(oe));
+        const uint64_t want = std::min<uint64_t>(65535, std::max<uint64_t>(1, (uint64_t)ctx->sm_count * std::max(resident, 1) / col_blocks));
         a.slice = std::max<uint64_t>(16, (a.n + want - 1) / want);
         const uint64_t slices = (a.n + a.slice - 1) / a.slice;
         if (rc == DPB_OK && slices > 1) rc = device_alloc(ctx, slices * 2 * width * sizeof(E), &parts);
@@ -265,7 +270,9 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
             e = cudaMemsetAsync(m->ptr, 0, m->len * sizeof(E), ctx->stream);  // keys without rows, and the padding
             if (e == cudaSuccess && a.n) {
                 const dim3 grid((uint32_t)col_blocks, (uint32_t)slices);
-                if (weights) row_products_kernel<F><<<grid, kRowSumThreads, 0, ctx->stream>>>(a, scale, scaled);
+                if (weights && (width & 1) == 0 && ((uintptr_t)a.x & 15) == 0)
+                    row_products_kernel<F, true><<<grid, kRowSumThreads, 0, ctx->stream>>>(a, scale, scaled);
+                else if (weights) row_products_kernel<F, false><<<grid, kRowSumThreads, 0, ctx->stream>>>(a, scale, scaled);
                 else row_sums_kernel<F><<<grid, kRowSumThreads, 0, ctx->stream>>>(a, scale, scaled);
                 if (slices > 1) {
                     const dim3 join((uint32_t)((width + kRowSumThreads - 1) / kRowSumThreads), (uint32_t)slices);

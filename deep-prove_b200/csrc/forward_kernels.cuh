@@ -265,54 +265,72 @@ struct RowSumArgs {
     void* parts;  // [slice][2][width]
 };
 
-// An unreduced sum of (weight) * (integer) products, or of plain integers.  Entries that fit 32 bits, as quantised
-// values do, enter as x + 2^31, an unsigned word: a product is then 8 wide multiply-adds for BN254 (4 for the two words
-// of each Goldilocks component) with no sign to look at, and the sum is 2^31 times the sum of the weights too large,
-// which `shift_back` takes back when the key's run ends.  Wider entries enter by magnitude with the weight or its
-// negative, plus 2^31 times the weight so that the same correction applies.
-template <class F, bool W>
-struct RowAccum;
+// An unreduced sum of (weight) * (integer) products.  A weight's 32-bit words and an entry of up to 16 bits are exact in
+// a double, a product is at most 2^47 and kExactRows of them stay within 2^53: the sums run as one fused multiply-add per
+// word on the 64-bit floating-point pipe, exactly, and move to signed 64-bit integers every kExactRows rows.  Wide integer
+// multiply-adds run at half a double's rate, and came with as many moves: 8192 rows of 4096 over BN254 took 88 us in a
+// chain of carries, 76 us in one 64-bit accumulator per word, and take 63 us this way.  What bounds it then is shared
+// between the weights' and entries' way through shared memory (57 % of its wavefronts) and the instructions' issue (59 %).
+// What an entry has above 16 bits, as quantised activations do not, takes a field product.
+constexpr uint32_t kExactRows = 64;
+// an integer below 2^31 in magnitude as a double, by its place next to 2^52
+__device__ __forceinline__ double exact_double(int32_t x) {
+    return __hiloint2double(0x43300000, x ^ (int32_t)0x80000000) - 4503601774854144.0;  // 2^52 + 2^31
+}
+__device__ __forceinline__ double exact_double(uint32_t x) { return __hiloint2double(0x43300000, (int32_t)x) - 4503599627370496.0; }
+template <class F>
+struct RowWords;
 template <>
-struct RowAccum<FrFam, true> {
-    frw::RowAcc s;  // below 2^286 per term: the words above 7 count carries only, so their 32 bits hold any run
-    __device__ __forceinline__ void zero() { s = frw::rowacc_zero(); }
-    __device__ __forceinline__ void mac32(const frw::F8& w, int32_t x) { frw::rowacc_mac(s, w.w, (uint32_t)x ^ 0x80000000u); }
-    static __device__ __forceinline__ frw::F8 weight(const Fr& w) { return frw::from_fr(w); }
-    // the sum, `more` added, as a field element; wsum = the sum of the weights
-    __device__ __forceinline__ Fr finish(const Fr& wsum, const Fr& more) const {
-        FrIntAcc t;
+struct RowWords<FrFam> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void cut(const Fr& w, double* out) {
+        const frw::F8 v = frw::from_fr(w);
 #pragma unroll
-        for (int i = 0; i < 12; i++) {
-            t.a.E[i] = i <= 8 ? s.E[i] : 0;
-            t.a.O[i] = i <= 9 ? s.O[i] : 0;
+        for (int j = 0; j < 8; j++) out[j] = exact_double(v.w[j]);
+    }
+    // sum_j a_j 2^(32 j), signed
+    static __device__ __forceinline__ Fr value(const int64_t* a) {
+        frw::F8 lo, hi;
+        int64_t carry = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int64_t v = a[j] + carry;
+            lo.w[j] = (uint32_t)v;
+            carry = v >> 32;
+            hi.w[j] = 0;
         }
-        frw::intacc_mac_lo(t.a, frw::from_fr(fr_neg(wsum)), 0x80000000u);
-        return fr_add(fr_intacc_finish(t), more);
+        const uint64_t mag = carry < 0 ? (uint64_t)0 - (uint64_t)carry : (uint64_t)carry;
+        hi.w[0] = (uint32_t)mag;
+        hi.w[1] = (uint32_t)(mag >> 32);
+        // lo + 2^256 hi: see fr_intacc_finish
+        const Fr l = frw::to_fr(frw::mul(lo, frw::from_fr(fr_one()))), h = frw::to_fr(frw::mul(hi, frw::from_fr(fr_rr())));
+        return carry < 0 ? fr_sub(l, h) : fr_add(l, h);
     }
 };
 template <>
-struct RowAccum<GlFam, true> {
-    glw::A8 s0, s1;
-    __device__ __forceinline__ void zero() { s0 = s1 = glw::acc_zero(); }
-    static __device__ __forceinline__ void mac(glw::A8& s, const glw::W& w, uint32_t u) {
-        asm("mad.lo.cc.u32 %0, %6, %8, %0; madc.hi.cc.u32 %1, %6, %8, %1; addc.u32 %2, %2, 0;\n\t"
-            "mad.lo.cc.u32 %3, %7, %8, %3; madc.hi.cc.u32 %4, %7, %8, %4; addc.u32 %5, %5, 0;"
-            : "+r"(s.e0), "+r"(s.e1), "+r"(s.e2), "+r"(s.o1), "+r"(s.o2), "+r"(s.o3)
-            : "r"(w.lo), "r"(w.hi), "r"(u));
+struct RowWords<GlFam> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void cut(const Gl2& w, double* out) {
+        const glw::W2 v = gl2_words(w);
+        out[0] = exact_double(v.c0.lo);
+        out[1] = exact_double(v.c0.hi);
+        out[2] = exact_double(v.c1.lo);
+        out[3] = exact_double(v.c1.hi);
     }
-    __device__ __forceinline__ void mac32(const glw::W2& w, int32_t x) {
-        mac(s0, w.c0, (uint32_t)x ^ 0x80000000u);
-        mac(s1, w.c1, (uint32_t)x ^ 0x80000000u);
+    static __device__ __forceinline__ uint64_t component(int64_t a0, int64_t a1) {
+        const int64_t v1 = a1 + (a0 >> 32), top = v1 >> 32;  // the number: top 2^64 + (v1's low word, a0's low word)
+        const uint64_t mag = top < 0 ? (uint64_t)0 - (uint64_t)top : (uint64_t)top;
+        glw::A5 l, h;
+        l.w0 = (uint32_t)a0;
+        l.w1 = (uint32_t)v1;
+        l.w2 = l.w3 = l.w4 = 0;
+        h.w0 = h.w1 = h.w4 = 0;
+        h.w2 = (uint32_t)mag;
+        h.w3 = (uint32_t)(mag >> 32);
+        const uint64_t lv = glw::to_u64(glw::canon(glw::acc_reduce(l))), hv = glw::to_u64(glw::canon(glw::acc_reduce(h)));
+        return top < 0 ? gl_sub(lv, hv) : gl_add(lv, hv);
     }
-    static __device__ __forceinline__ glw::W2 weight(const Gl2& w) { return gl2_words(w); }
-    __device__ __forceinline__ Gl2 finish(const Gl2& wsum, const Gl2& more) const {
-        glw::A8 t0 = s0, t1 = s1;
-        const glw::W2 n = gl2_words(gl2_neg(wsum));
-        // one more term; the words next to e1 and o2 count carries only, and no run has 2^32 terms
-        mac(t0, n.c0, 0x80000000u);
-        mac(t1, n.c1, 0x80000000u);
-        return GlFam::add(gl2_make(glw::to_u64(glw::canon(glw::acc_reduce(t0))), glw::to_u64(glw::canon(glw::acc_reduce(t1)))), more);
-    }
+    static __device__ __forceinline__ Gl2 value(const int64_t* a) { return gl2_make(component(a[0], a[1]), component(a[2], a[3])); }
 };
 template <class F>
 __device__ __forceinline__ typename F::E field_from_i128(__int128 v) {
@@ -323,12 +341,11 @@ __device__ __forceinline__ typename F::E field_from_i128(__int128 v) {
     return neg ? F::neg(r) : r;
 }
 
-// v += w * (x - its low 32 bits as a signed word), for the rare entry that has more than those
+// v + w * (x - its low 16 bits, signed)
 template <class F>
 __device__ __noinline__ typename F::E add_high(typename F::E v, const typename F::E w, int64_t x) {
-    const int64_t hi = (x >> 32) + ((int32_t)x < 0 ? 1 : 0);
-    if (hi == 0) return v;
-    const typename F::E t = F::mul(w, F::mul(F::from_u64(hi < 0 ? (uint64_t)0 - (uint64_t)hi : (uint64_t)hi), F::from_u64(1ull << 32)));
+    const int64_t hi = (x >> 16) + ((x >> 15) & 1);  // x = its low 16 bits, signed, + 2^16 hi
+    const typename F::E t = F::mul(w, F::mul(F::from_u64(hi < 0 ? (uint64_t)0 - (uint64_t)hi : (uint64_t)hi), F::from_u64(1ull << 16)));
     return hi < 0 ? F::sub(v, t) : F::add(v, t);
 }
 
@@ -336,104 +353,140 @@ __device__ __noinline__ typename F::E add_high(typename F::E v, const typename F
 // prefix sums, go through shared memory; kRowSumFlight rows' entries are loaded ahead of the products.
 constexpr uint32_t kRowSumThreads = 128, kRowSumBatch = 64, kRowSumFlight = 8;
 
-// two neighbouring columns per thread with weights (a weight read from shared memory then serves two products)
-template <class F>
-__global__ void __launch_bounds__(kRowSumThreads)
+// With weights: two columns per thread (a weight read from shared memory then serves two products).  The entries come
+// through a per-thread ring in shared memory, kRingAhead groups of four rows ahead of the products, so that loads are
+// under way all the time.
+constexpr uint32_t kRowRing = 4, kRingAhead = kRowRing - 1, kProductBatch = 128;
+template <int BYTES>
+__device__ __forceinline__ void ring_load(void* dst, const void* src) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+// PAIRS: rows of an even number of entries at 16-byte addresses, so that a thread's two columns are one word
+template <class F, bool PAIRS>
+__global__ void __launch_bounds__(kRowSumThreads, sizeof(typename F::E) == 32 ? 4 : 5)
     row_products_kernel(RowSumArgs a, typename F::E multiplier, bool scale) {
     typedef typename F::E E;
-    constexpr int C = 2;
-    __shared__ E wsh[kRowSumBatch], prefix[kRowSumBatch];
-    __shared__ uint64_t at[kRowSumBatch];
-    __shared__ uint32_t keys[kRowSumBatch];
-    __shared__ uint32_t ends[kRowSumBatch / 32];  // a bit per row: the key's run ends here
-    const uint64_t c0 = (uint64_t)blockIdx.x * (kRowSumThreads * C) + threadIdx.x;
+    constexpr int C = 2, N = RowWords<F>::N;
+    __shared__ __align__(16) double wsh[kProductBatch + 1][N];  // the last weight is zero
+    __shared__ longlong2 ring[kRowRing][4][kRowSumThreads];
+    __shared__ const int64_t* from[kProductBatch];
+    __shared__ uint32_t keys[kProductBatch];
+    __shared__ uint32_t ends[kProductBatch / 32];  // a bit per row: the key's run ends here
+    const uint32_t tid = threadIdx.x, lane = tid & 31;
+    const uint64_t c0 = ((uint64_t)blockIdx.x * kRowSumThreads + tid) * C;
     const uint64_t begin = blockIdx.y * a.slice, end = begin + a.slice < a.n ? begin + a.slice : a.n;
-    const uint32_t lane = threadIdx.x & 31;
-    bool live[C];
-#pragma unroll
-    for (int q = 0; q < C; q++) live[q] = c0 + q * kRowSumThreads < a.width;
+    const bool live[C] = {c0 < a.width, c0 + 1 < a.width};
+    // columns past the last read some column's entries, and keep the result to themselves
+    const uint64_t c_load = live[0] ? c0 : 0, second = live[1] ? 1 : 0;
+    if (tid < N) wsh[kProductBatch][tid] = 0.0;
     bool before = begin > 0 && a.keys[begin - 1] == a.keys[begin];  // the current run began before the slice
-    RowAccum<F, true> acc[C];
-    E wide[C];  // what the entries of more than 32 bits add (seldom any)
+    double acc[C][N];
+    int64_t sum[C][N];
+    E wide[C];  // what the entries of more than 16 bits add (seldom any)
     bool any_wide = false;
 #pragma unroll
     for (int q = 0; q < C; q++) {
-        acc[q].zero();
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            acc[q][j] = 0.0;
+            sum[q][j] = 0;
+        }
         wide[q] = F::zero();
     }
-    E run_weights = F::zero();  // of the run's rows in earlier batches
-    for (uint64_t p0 = begin; p0 < end; p0 += kRowSumBatch) {
-        const uint32_t m = end - p0 < kRowSumBatch ? (uint32_t)(end - p0) : kRowSumBatch;
-        __syncthreads();
-        if (threadIdx.x < kRowSumBatch) {
-            const uint32_t i = threadIdx.x < m ? threadIdx.x : m - 1;
-            const uint64_t p = p0 + i;
-            const uint32_t row = a.rows[p], key = a.keys[p];
-            at[threadIdx.x] = (uint64_t)(row / a.per) * a.width;
-            keys[threadIdx.x] = key;
-            const uint32_t run_ends = __ballot_sync(0xffffffffu, threadIdx.x < m && (p + 1 == end || a.keys[p + 1] != key));
-            if (lane == 0) ends[threadIdx.x >> 5] = run_ends;
-            const E w = F::load(a.weights, F::kChalDtype, row);
-            wsh[threadIdx.x] = w;
-            E sum = w;
+    auto drain = [&]() {
 #pragma unroll
-            for (int off = 1; off < 32; off <<= 1) {
-                const E o = F::shfl_up(sum, off);
-                if (lane >= (uint32_t)off) sum = F::add(sum, o);
+        for (int q = 0; q < C; q++)
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                sum[q][j] += (int64_t)acc[q][j];
+                acc[q][j] = 0.0;
             }
-            prefix[threadIdx.x] = sum;
+    };
+    for (uint64_t p0 = begin; p0 < end; p0 += kProductBatch) {
+        const uint32_t m = end - p0 < kProductBatch ? (uint32_t)(end - p0) : kProductBatch;
+        __syncthreads();
+        {
+            const uint64_t p = p0 + (tid < m ? tid : m - 1);
+            const uint32_t row = a.rows[p], key = a.keys[p];
+            from[tid] = a.x + (uint64_t)(row / a.per) * a.width;
+            keys[tid] = key;
+            const uint32_t run_ends = __ballot_sync(0xffffffffu, tid < m && (p + 1 == end || a.keys[p + 1] != key));
+            if (lane == 0) ends[tid >> 5] = run_ends;
+            RowWords<F>::cut(F::load(a.weights, F::kChalDtype, row), wsh[tid]);
         }
         __syncthreads();
-        // the weights of rows s..i of the batch: the prefix sums run inside each half of 32
-        auto weights_of = [&](uint32_t s, uint32_t i) {
-            E v = prefix[i];
-            if (s < 32 && i >= 32) v = F::add(v, prefix[31]);
-            if (s & 31) v = F::sub(v, prefix[s - 1]);
-            return v;
-        };
-        // one run, or the part of it in this batch, after the other; the loop over its rows holds the products alone, so
-        // that it stays in the instruction cache (with the ends of runs unrolled into it: 158 us instead of 37)
-        const uint64_t run_ends = ends[0] | (uint64_t)ends[1] << 32;
-        for (uint32_t s = 0; s < m;) {
-            const uint64_t rest = run_ends >> s;
-            const uint32_t t = rest ? s + __ffsll(rest) - 1 : m - 1;  // the run's last row here
-            for (uint32_t i0 = s; i0 <= t; i0 += kRowSumFlight) {
-                int64_t x[kRowSumFlight][C];
-                int64_t high = 0;
+        auto issue = [&](uint32_t g) {
+            if (4 * g < m) {
+                longlong2* dst = &ring[g % kRowRing][0][tid];
 #pragma unroll
-                for (uint32_t u = 0; u < kRowSumFlight; u++)
-#pragma unroll
-                    for (int q = 0; q < C; q++)
-                        x[u][q] = live[q] && i0 + u <= t ? __ldg((const long long*)a.x + at[i0 + u] + c0 + q * kRowSumThreads) : 0;
-#pragma unroll
-                for (uint32_t u = 0; u < kRowSumFlight; u++) {
-                    if (i0 + u > t) break;
-                    const auto w = RowAccum<F, true>::weight(wsh[i0 + u]);
-#pragma unroll
-                    for (int q = 0; q < C; q++) {
-                        acc[q].mac32(w, (int32_t)x[u][q]);
-                        high |= x[u][q] - (int32_t)x[u][q];
+                for (uint32_t u = 0; u < 4; u++) {  // rows past the batch's last repeat that one
+                    const int64_t* src = from[4 * g + u] + c_load;
+                    if (PAIRS) {
+                        ring_load<16>(dst + u * kRowSumThreads, src);
+                    } else {
+                        ring_load<8>(&dst[u * kRowSumThreads].x, src);
+                        ring_load<8>(&dst[u * kRowSumThreads].y, src + second);
                     }
                 }
-                if (high) {
-                    any_wide = true;
-#pragma unroll 1
-                    for (uint32_t u = 0; u < kRowSumFlight && i0 + u <= t; u++)
-#pragma unroll
-                        for (int q = 0; q < C; q++)
-                            if (live[q]) wide[q] = add_high<F>(wide[q], wsh[i0 + u], a.x[at[i0 + u] + c0 + q * kRowSumThreads]);
-                }
             }
-            const E ws = weights_of(s, t);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (uint32_t g = 0; g < kRingAhead; g++) issue(g);
+        uint32_t next = 0;  // the first group that was not waited for
+        // One run, or the part of it in this batch, after the other.  The loop over its rows holds the products alone: with
+        // the ends of runs unrolled into it, it left the instruction cache.
+        for (uint32_t s = 0; s < m;) {
+            uint32_t h = s >> 5, rest = ends[h] >> (s & 31) << (s & 31);
+            while (!rest && ++h < kProductBatch / 32) rest = ends[h];
+            const uint32_t t = rest ? 32 * h + __ffs(rest) - 1 : m - 1;  // the run's last row here
+            for (uint32_t g = s >> 2; g <= t >> 2; g++) {
+                if (g == next) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kRingAhead - 1) : "memory");
+                    issue(g + kRingAhead);  // into the group before this one, whose products are done
+                    next++;
+                }
+                bool more = false;  // an entry has more than 16 bits
+                const longlong2* x4 = &ring[g % kRowRing][0][tid];
+#pragma unroll
+                for (uint32_t u = 0; u < 4; u++) {
+                    const uint32_t i = 4 * g + u;
+                    const double* w = wsh[i >= s && i <= t ? i : kProductBatch];  // other runs' rows: times 0
+                    const longlong2 x2 = x4[u * kRowSumThreads];
+#pragma unroll
+                    for (int q = 0; q < C; q++) {
+                        const int64_t x = q ? x2.y : x2.x;
+                        more |= x != (int64_t)(int16_t)x;
+                        const double d = exact_double((int32_t)(int16_t)x);
+#pragma unroll
+                        for (int j = 0; j < N; j++) acc[q][j] = fma(w[j], d, acc[q][j]);
+                    }
+                }
+                if (more) {
+#pragma unroll 1
+                    for (uint32_t i = max(s, 4 * g); i <= min(t, 4 * g + 3); i++) {
+                        const E w = F::load(a.weights, F::kChalDtype, a.rows[p0 + i]);
+                        const longlong2 x2 = x4[(i & 3) * kRowSumThreads];
+                        wide[0] = add_high<F>(wide[0], w, x2.x);
+                        wide[1] = add_high<F>(wide[1], w, x2.y);
+                    }
+                    any_wide = true;
+                }
+                if (g % (kExactRows / 4) == kExactRows / 4 - 1) drain();
+            }
+            drain();
             if (rest) {
                 const uint32_t key = keys[t];
                 const bool after = p0 + t + 1 == end && end < a.n && a.keys[end] == key;
-                const E total = F::add(run_weights, ws);
 #pragma unroll
                 for (int q = 0; q < C; q++) {
                     if (live[q]) {
-                        const uint64_t c = c0 + q * kRowSumThreads;
-                        E v = acc[q].finish(total, wide[q]);
+                        const uint64_t c = c0 + q;
+                        E v = RowWords<F>::value(sum[q]);
+                        if (any_wide) v = F::add(v, wide[q]);
                         if (before || after) {
                             F::store(a.parts, ((uint64_t)blockIdx.y * 2 + (before ? 0 : 1)) * a.width + c, v);
                         } else {
@@ -441,20 +494,16 @@ __global__ void __launch_bounds__(kRowSumThreads)
                             F::store(a.out, (uint64_t)key * a.out_width + c, v);
                         }
                     }
-                }
 #pragma unroll
-                for (int q = 0; q < C; q++) {
-                    acc[q].zero();
+                    for (int j = 0; j < N; j++) sum[q][j] = 0;
                     if (any_wide) wide[q] = F::zero();
                 }
                 any_wide = false;
                 before = false;
-                run_weights = F::zero();
-            } else {
-                run_weights = F::add(run_weights, ws);
             }
             s = t + 1;
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
 }
 
