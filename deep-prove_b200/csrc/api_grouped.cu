@@ -13,16 +13,17 @@ static cudaError_t launch_product(dpb_ctx* ctx, const GroupedArgs& a, uint32_t b
     const uint32_t smem = GroupedShape<XD, WD, T>::smem(a.n_experts);
     cudaError_t e = cudaFuncSetAttribute(grouped_product_kernel<XD, WD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    grouped_product_kernel<XD, WD, T><<<blocks, 192, smem, ctx->stream>>>(a);
+    grouped_product_kernel<XD, WD, T><<<blocks, kGroupedThreads, smem, ctx->stream>>>(a);
     return cudaGetLastError();
 }
 template <int XD, int WD>
-static cudaError_t launch_rows(dpb_ctx* ctx, const GroupedArgs& a, uint32_t rows_log2, uint32_t blocks) {
-    switch (rows_log2) {
-        case 4: return launch_product<XD, WD, 16>(ctx, a, blocks);
-        case 5: return launch_product<XD, WD, 32>(ctx, a, blocks);
-        case 6: return launch_product<XD, WD, 64>(ctx, a, blocks);
-        default: return launch_product<XD, WD, 128>(ctx, a, blocks);
+static cudaError_t launch_rows(dpb_ctx* ctx, const GroupedArgs& a, uint32_t rows, uint32_t blocks) {
+    switch (rows) {
+        case 16: return launch_product<XD, WD, 16>(ctx, a, blocks);
+        case 32: return launch_product<XD, WD, 32>(ctx, a, blocks);
+        case 64: return launch_product<XD, WD, 64>(ctx, a, blocks);
+        case 128: return launch_product<XD, WD, 128>(ctx, a, blocks);
+        default: return launch_product<XD, WD, 160>(ctx, a, blocks);
     }
 }
 
@@ -68,13 +69,16 @@ static int product_impl(dpb_ctx* ctx, int dtype, const dpb_row_groups* g, const 
     void *owned = nullptr, *planes = nullptr;
     int rc = fwd_check_begin(ctx, &check);
     if (rc == DPB_OK) rc = fwd_tensor(ctx, x, x_on_device, n / per * w->inner, &dev, &owned);
-    // Rows per tile: what an expert gets on average, so that a tile's columns of the instruction are mostly used; an
-    // instruction of 128 rows takes as long as its operands' way to the tensor cores either way
+    // Rows per tile.  An instruction takes as long for 16 rows as for 128 (about 70 clocks; 85 for 160), so a tile should
+    // hold what an expert gets: fewer, fuller tiles read the weights less often.  Small tiles leave room for more stages
+    // (few rows: bound by the weights' way from HBM) and, up to 64 rows of two digits, for a second accumulator.
+    // Measured: 52 rows per expert 24.9 us with 64, 25.9 with 128; 128 rows 61 us with 128, 67 with 64 or 160; 2048 rows
+    // 1.95 ms with 160, 2.20 with 128, 3.45 with 64.
     const uint64_t used = std::min<uint64_t>(w->n_experts, n), average = (n + used - 1) / used;
-    const uint32_t rows_log2 = average <= 16 ? 4 : average <= 32 ? 5 : average <= 64 ? 6 : 7;
-    const uint64_t max_tiles = (n >> rows_log2) + used;  // every expert's last tile may be partly filled
+    const uint32_t T = average <= 8 ? 16 : average <= 16 ? 32 : average <= 64 ? 64 : average < 320 ? 128 : 160;
+    const uint64_t max_tiles = n / T + used;  // every expert's last tile may be partly filled
     const uint32_t digits = digits_of(x_bits);
-    if (rc == DPB_OK) rc = device_alloc(ctx, max_tiles * w->k_blocks * digits * (128ull << rows_log2), &planes);
+    if (rc == DPB_OK) rc = device_alloc(ctx, max_tiles * w->k_blocks * digits * 128 * T, &planes);
     cudaError_t e = cudaSuccess;
     unsigned int found = 0;
     if (rc == DPB_OK) {
@@ -84,10 +88,10 @@ static int product_impl(dpb_ctx* ctx, int dtype, const dpb_row_groups* g, const 
         const int64_t half = 1ll << (x_bits - 1);
         if (digits == 1)
             cut_rows_kernel<1><<<blocks, kCutThreads, smem, ctx->stream>>>(dev, g->keys, g->places, g->offsets, n / per, per, w->n_experts, w->inner,
-                                                                           w->k_blocks, rows_log2, half, (int8_t*)planes, check);
+                                                                           w->k_blocks, T, half, (int8_t*)planes, check);
         else
             cut_rows_kernel<2><<<blocks, kCutThreads, smem, ctx->stream>>>(dev, g->keys, g->places, g->offsets, n / per, per, w->n_experts, w->inner,
-                                                                           w->k_blocks, rows_log2, half, (int8_t*)planes, check);
+                                                                           w->k_blocks, T, half, (int8_t*)planes, check);
         e = cudaGetLastError();
         GroupedArgs a;
         memset(&a, 0, sizeof a);
@@ -103,16 +107,16 @@ static int product_impl(dpb_ctx* ctx, int dtype, const dpb_row_groups* g, const 
         a.gave_up = fwd_gave_up_word(ctx);
         // When the tiles are fewer than four rounds of the GPU's blocks, the inner dimension is cut as well, into items
         // of at least four stages: a block's last item then costs little, and few tiles still keep every SM reading
-        const uint64_t tiles = ((n >> rows_log2) + (used + 1) / 2) * w->col_tiles;
-        uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>(w->k_blocks / 4, (uint64_t)ctx->sm_count * 4 / std::max<uint64_t>(tiles, 1)));
+        const uint64_t tiles = (n / T + (used + 1) / 2) * w->col_tiles, workers = ctx->sm_count;
+        uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>(w->k_blocks / 4, workers * 4 / std::max<uint64_t>(tiles, 1)));
         splits = std::max<uint64_t>(splits, (w->k_blocks + kMaxSteps - 1) / kMaxSteps);
         a.blocks_per_split = (uint32_t)((w->k_blocks + splits - 1) / splits);
         a.splits = (w->k_blocks + a.blocks_per_split - 1) / a.blocks_per_split;
         if (e == cudaSuccess && a.splits > 1) e = cudaMemsetAsync(a.out, 0, n * w->cols * 8, ctx->stream);
-        const uint32_t grid = (uint32_t)std::min<uint64_t>(max_tiles * w->col_tiles * a.splits, (uint64_t)ctx->sm_count);
+        const uint32_t grid = (uint32_t)std::min<uint64_t>(max_tiles * w->col_tiles * a.splits, workers);
         if (e == cudaSuccess) {
-            if (digits == 1) e = w->digits == 1 ? launch_rows<1, 1>(ctx, a, rows_log2, grid) : launch_rows<1, 2>(ctx, a, rows_log2, grid);
-            else e = w->digits == 1 ? launch_rows<2, 1>(ctx, a, rows_log2, grid) : launch_rows<2, 2>(ctx, a, rows_log2, grid);
+            if (digits == 1) e = w->digits == 1 ? launch_rows<1, 1>(ctx, a, T, grid) : launch_rows<1, 2>(ctx, a, T, grid);
+            else e = w->digits == 1 ? launch_rows<2, 1>(ctx, a, T, grid) : launch_rows<2, 2>(ctx, a, T, grid);
         }
         rc = e == cudaSuccess ? fwd_check_wait(ctx, check, &found) : fail(DPB_ECUDA, "grouped product: %s", cudaGetErrorString(e));
     }

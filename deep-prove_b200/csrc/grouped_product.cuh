@@ -10,6 +10,11 @@
 // The weights' 128 columns are the instruction's M (rows of the accumulator = TMEM lanes) and a tile's routed rows its
 // N: a warp's lanes then hold neighbouring columns of one output row, which is stored as whole 256-byte runs without a
 // transposition, and a tile of few rows (a single token) wastes nothing.
+//
+// What bounds it.  Many rows: the instruction, at two per 8-bit pair's worth of 16-bit work; 16384 routed rows of 4096 by
+// 8 matrices of 4096 x 11008 take 1.95 ms, 5.9e12 digit operations at 3.0 P/s against 3.3 P/s (twice the measured bf16
+// rate), with the power cap at work.  Two blocks sharing a tile (cta_group::2) brought less through L2 but took 2.02 ms.
+// One token through two experts: the weights' 180 MB from HBM, 37 us against 28.
 #pragma once
 #include "forward.cuh"
 
@@ -84,14 +89,13 @@ __global__ void __launch_bounds__(kCutThreads)
 }
 
 // first tile of every expert: tiles[e] = sum of ceil(rows / T) over the experts before e
-__device__ __forceinline__ void expert_tiles(const uint32_t* __restrict__ offsets, uint32_t n_experts, uint32_t rows_log2,
+__device__ __forceinline__ void expert_tiles(const uint32_t* __restrict__ offsets, uint32_t n_experts, uint32_t T,
                                              uint32_t* tiles /* shared, n_experts + 1 */) {
-    const uint32_t T1 = (1u << rows_log2) - 1;
     if (threadIdx.x < 32) {
         uint32_t carry = 0;
         for (uint32_t e0 = 0; e0 < n_experts; e0 += 32) {
             const uint32_t e = e0 + threadIdx.x;
-            const uint32_t n = e < n_experts ? (offsets[e + 1] - offsets[e] + T1) >> rows_log2 : 0;
+            const uint32_t n = e < n_experts ? (offsets[e + 1] - offsets[e] + T - 1) / T : 0;
             uint32_t incl = n;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
@@ -114,13 +118,13 @@ template <int DIGITS>
 __global__ void __launch_bounds__(kCutThreads)
     cut_rows_kernel(const int64_t* __restrict__ x, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ places,
                     const uint32_t* __restrict__ offsets, uint64_t tokens, uint32_t per, uint32_t n_experts, uint64_t inner,
-                    uint32_t k_blocks, uint32_t rows_log2, int64_t half, int8_t* __restrict__ planes, FwdCheck check) {
+                    uint32_t k_blocks, uint32_t T, int64_t half, int8_t* __restrict__ planes, FwdCheck check) {
     extern __shared__ uint32_t tiles[];
     __shared__ __align__(16) uint8_t cut[kCutThreads / 32][DIGITS][kCutEntries];
     unsigned int found = 0;
-    expert_tiles(offsets, n_experts, rows_log2, tiles);
+    expert_tiles(offsets, n_experts, T, tiles);
     __syncthreads();
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, T = 1u << rows_log2;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t per_row = (k_blocks + 1) / 2;  // 256 entries = two stages
     const uint64_t total = tokens * per_row, step = (uint64_t)gridDim.x * (kCutThreads / 32);
     for (uint64_t t = (uint64_t)blockIdx.x * (kCutThreads / 32) + warp; t < total; t += step) {
@@ -145,9 +149,9 @@ __global__ void __launch_bounds__(kCutThreads)
         if (digit < DIGITS && block < k_blocks) {
             const uint4 bytes = *(const uint4*)&cut[warp][digit][16 * piece];
             for (uint32_t j = 0; j < per; j++) {
-                const uint32_t p = places[token * per + j], e = keys[p], at = p - offsets[e];
-                const uint64_t tile = (uint64_t)(tiles[e] + (at >> rows_log2)) * k_blocks + block;
-                *(uint4*)(planes + (tile * DIGITS + digit) * (T * 128) + tile_piece(at & (T - 1), piece & 7)) = bytes;
+                const uint32_t p = places[token * per + j], e = keys[p], at = p - offsets[e], q = at / T;
+                const uint64_t tile = (uint64_t)(tiles[e] + q) * k_blocks + block;
+                *(uint4*)(planes + (tile * DIGITS + digit) * (T * 128) + tile_piece(at - q * T, piece & 7)) = bytes;
             }
         }
         __syncwarp();
@@ -172,15 +176,27 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// Waits for the phase; gives up (and tells the block's other roles) after kWaitTries tries, seconds at the least.
-constexpr uint32_t kWaitTries = 1u << 24;
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-    for (uint32_t i = 0; i < kWaitTries; i++) {
-        if (bar_try(bar, parity)) return true;
+// Waits for the phase; gives up, and tells the block's other roles, after kWaitNs.
+constexpr uint64_t kWaitNs = 5ull * 1000 * 1000 * 1000;
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+template <class Try>
+__device__ __forceinline__ bool wait_limited(Try once, volatile int* gave_up) {
+    if (once()) return true;
+    const uint64_t t0 = now_ns();
+    for (uint32_t i = 1;; i++) {
+        if (once()) return true;
         if (*gave_up) return false;
+        if ((i & 63) == 0 && now_ns() - t0 > kWaitNs) break;
     }
     *gave_up = 1;
     return false;
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+    return wait_limited([&]() { return bar_try(bar, parity); }, gave_up);
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
@@ -232,13 +248,77 @@ struct GroupedShape {
     static constexpr uint32_t smem(uint32_t n_experts) { return kStages * kStageBytes + 1024 + (n_experts + 1) * 4; }
 };
 
-// Six warps: 0-3 move finished accumulators to the output, 4 brings the operands, 5 issues the products.  One block per
+// The eight warps that move a finished tile: warp w reads the accumulators' lanes 32 (w mod 4) .. + 31, that is 32
+// columns, and of the rows the sixteens w / 4, w / 4 + 2, ...  Accumulators wait for this when there is room for one
+// tile's only, so it is kept short: the rows' places in the output are read before the tile is finished (tile_rows), and
+// a sixteen's accumulators are on their way while the last one's results are stored.
+constexpr uint32_t kStoreWarps = 8, kGroupedThreads = 32 * (kStoreWarps + 2);
+template <int T>
+struct TileRows {
+    uint32_t row[(T + 31) / 32];  // lane l: rows l, l + 32, ... of the tile
+    __device__ __forceinline__ void load(const uint32_t* __restrict__ rows, uint32_t lo, int valid) {
+#pragma unroll
+        for (int i = 0; i < (T + 31) / 32; i++) {
+            const int j = 32 * i + (threadIdx.x & 31);
+            row[i] = j < valid ? rows[lo + j] : 0;
+        }
+    }
+};
+// accumulators -> 64-bit results; `release` is called when the warp has read its accumulators
+template <int ACC, int T, class Release>
+__device__ __forceinline__ void store_tile(const GroupedArgs& a, uint32_t acc, const TileRows<T>& rows, int valid, uint64_t c,
+                                           uint32_t half, Release release) {
+    constexpr int kChunks = (T + 31) / 32;
+    uint32_t r[2][ACC][16];
+    const int mine = (valid - 16 * (int)half + 31) / 32;  // sixteens of this warp with a row in them
+    auto read = [&](int i) {
+#pragma unroll
+        for (int d = 0; d < ACC; d++) tmem_load16(acc + d * T + 32 * i + 16 * half, r[i & 1][d]);
+    };
+    auto done_reading = [&]() {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        release();
+    };
+    if (mine > 0) read(0);
+    else done_reading();
+#pragma unroll
+    for (int i = 0; i < kChunks; i++) {
+        if (i >= mine) break;
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (i + 1 < kChunks && i + 1 < mine) read(i + 1);
+        else done_reading();
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const uint32_t row = __shfl_sync(0xffffffffu, rows.row[i], 16 * half + j);
+            int64_t y = (int32_t)r[i & 1][0][j];
+#pragma unroll
+            for (int d = 1; d < ACC; d++) y += (int64_t)(int32_t)r[i & 1][d][j] << (8 * d);
+            if (c < a.cols && 32 * i + 16 * (int)half + j < valid) {
+                int64_t* o = a.out + (uint64_t)row * a.cols + c;
+                if (a.splits > 1) atomicAdd((unsigned long long*)o, (unsigned long long)y);
+                else __stcs((long long*)o, (long long)y);
+            }
+        }
+    }
+}
+
+// After a wait that ran out: the host learns of it, and copies and products in flight must not outlive the block, so it
+// stays for a second.  Called by the whole block.
+__device__ __forceinline__ void gave_up_wait(unsigned int* word) {
+    if (threadIdx.x == 0) {
+        *(volatile unsigned int*)word = 1;
+        for (uint32_t t = 0; t < (1u << 20); t++) __nanosleep(1000);
+    }
+    __syncthreads();
+}
+
+// Ten warps: 0-7 move finished accumulators to the output, 8 brings the operands, 9 issues the products.  One block per
 // SM walks the work items blockIdx.x, + gridDim.x, ...; items of one expert are ordered with the row tiles fastest, so
 // that the blocks at work at one time share the weights' and rows' tiles in L2.
 template <int XD, int WD, int T>
-__global__ void __launch_bounds__(192, 1) grouped_product_kernel(GroupedArgs a) {
+__global__ void __launch_bounds__(kGroupedThreads, 1) grouped_product_kernel(GroupedArgs a) {
     typedef GroupedShape<XD, WD, T> S;
-    constexpr uint32_t rows_log2 = T == 16 ? 4 : T == 32 ? 5 : T == 64 ? 6 : 7;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t bars[2 * S::kStages + 4];
     __shared__ uint32_t tmem_slot;
@@ -251,7 +331,7 @@ __global__ void __launch_bounds__(192, 1) grouped_product_kernel(GroupedArgs a) 
     auto empty = [&](uint32_t s) { return bar0 + 8 * (S::kStages + s); };
     auto acc_full = [&](uint32_t b) { return bar0 + 8 * (2 * S::kStages + b); };
     auto acc_empty = [&](uint32_t b) { return bar0 + 8 * (2 * S::kStages + 2 + b); };
-    expert_tiles(a.offsets, a.n_experts, rows_log2, tiles);
+    expert_tiles(a.offsets, a.n_experts, T, tiles);
     if (threadIdx.x == 0) {
         gave_up = 0;
         for (uint32_t s = 0; s < S::kStages; s++) {
@@ -260,12 +340,12 @@ __global__ void __launch_bounds__(192, 1) grouped_product_kernel(GroupedArgs a) 
         }
         for (uint32_t b = 0; b < 2; b++) {
             bar_init(acc_full(b), 1);
-            bar_init(acc_empty(b), 4);
+            bar_init(acc_empty(b), kStoreWarps);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 5) {
+    if (warp == kStoreWarps + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(S::kTmem)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -295,7 +375,7 @@ __global__ void __launch_bounds__(192, 1) grouped_product_kernel(GroupedArgs a) 
     };
 
     uint32_t e = 0;
-    if (warp == 4 && lane == 0) {
+    if (warp == kStoreWarps && lane == 0) {
         uint32_t stage = 0, phase = 0;
         for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {
             const Item it = item_at(i, e);
@@ -321,7 +401,7 @@ __global__ void __launch_bounds__(192, 1) grouped_product_kernel(GroupedArgs a) 
                 phase ^= 1;
             }
         }
-    } else if (warp == 5 && lane == 0) {
+    } else if (warp == kStoreWarps + 1 && lane == 0) {
         // D = S32, A and B = signed 8 bits, both K-major
         constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(T >> 3) << 17) | ((kTileCols >> 4) << 24);
         uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
@@ -357,39 +437,19 @@ __global__ void __launch_bounds__(192, 1) grouped_product_kernel(GroupedArgs a) 
                 buf_phase ^= 1;
             }
         }
-    } else if (warp < 4) {
+    } else if (warp < kStoreWarps) {
         uint32_t buf = 0, buf_phase = 0;
         for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {
             const Item it = item_at(i, e);
-            if (!bar_wait(acc_full(buf), buf_phase, &gave_up)) goto done;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t lo = a.offsets[e] + it.row_tile * T, end = a.offsets[e + 1];
             const int valid = end - lo < T ? (int)(end - lo) : T;
-            const uint64_t c = (uint64_t)it.col_tile * kTileCols + warp * 32 + lane;
-            const uint32_t acc = tmem + buf * (S::kAcc * T) + (warp << 21);
-            for (int j0 = 0; j0 < valid; j0 += 16) {
-                uint32_t r[S::kAcc][16];
-#pragma unroll
-                for (int d = 0; d < S::kAcc; d++) tmem_load16(acc + d * T + j0, r[d]);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (j0 + 16 >= valid) {  // the accumulators are in registers: the next tile's products may start
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(acc_empty(buf));
-                }
-                if (c < a.cols) {
-#pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        if (j0 + j >= valid) break;
-                        int64_t y = (int32_t)r[0][j];
-#pragma unroll
-                        for (int d = 1; d < S::kAcc; d++) y += (int64_t)(int32_t)r[d][j] << (8 * d);
-                        int64_t* o = a.out + (uint64_t)a.rows[lo + j0 + j] * a.cols + c;
-                        if (a.splits > 1) atomicAdd((unsigned long long*)o, (unsigned long long)y);
-                        else __stcs((long long*)o, (long long)y);
-                    }
-                }
-            }
+            const uint64_t c = (uint64_t)it.col_tile * kTileCols + (warp & 3) * 32 + lane;
+            TileRows<T> rows;
+            rows.load(a.rows, lo, valid);
+            if (!bar_wait(acc_full(buf), buf_phase, &gave_up)) goto done;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            store_tile<S::kAcc, T>(a, tmem + buf * (S::kAcc * T) + ((warp & 3) << 21), rows, valid, c, warp >> 2,
+                                   [&]() { if (lane == 0) bar_arrive(acc_empty(buf)); });
             if (++buf == S::kBuffers) {
                 buf = 0;
                 buf_phase ^= 1;
@@ -399,15 +459,8 @@ __global__ void __launch_bounds__(192, 1) grouped_product_kernel(GroupedArgs a) 
 done:
     __syncwarp();
     __syncthreads();
-    if (gave_up) {
-        // copies and products in flight must not outlive the block: wait for every stage that was asked for, with a limit
-        if (threadIdx.x == 0) {
-            *(volatile unsigned int*)a.gave_up = 1;
-            for (uint32_t t = 0; t < (1u << 20); t++) __nanosleep(1000);
-        }
-        __syncthreads();
-    }
-    if (warp == 5) {
+    if (gave_up) gave_up_wait(a.gave_up);
+    if (warp == kStoreWarps + 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kTmem));
     }

@@ -222,7 +222,7 @@ def check_product(ctx, fw, keys, x, w, xb, wb, per=1):
 
 @pytest.mark.parametrize("xb,wb", [(14, 12), (8, 12), (15, 8), (8, 8), (2, 2), (15, 15)])
 @pytest.mark.parametrize("n,experts,inner,cols", [(1, 1, 1, 1), (3, 2, 128, 128), (16, 1, 130, 129), (40, 3, 257, 100),
-                                                  (100, 2, 64, 300), (300, 2, 384, 65), (700, 4, 1100, 130)])
+                                                  (100, 2, 64, 300), (300, 2, 384, 65), (700, 4, 1100, 130), (999, 2, 150, 200)])
 def test_product(ctx, fw, xb, wb, n, experts, inner, cols):
     rng = np.random.default_rng(n + inner)
     x = rng.integers(-2**(xb - 1), 2**(xb - 1), size=(n, inner))
