@@ -354,6 +354,7 @@ static int fix_common(dpb_ctx* ctx, const dpb_mle* mle, const void* point, uint3
                       dpb_mle** out) {
     if (!ctx || !mle || !out || (!point && k)) return fail(DPB_EINVAL, "null argument");
     const uint32_t n = log2u(mle->len);
+    if (mle->len != (1ull << n)) return fail(DPB_EINVAL, "a table of %llu entries, not a power of two", (unsigned long long)mle->len);
     if (k == 0 || k > n) return fail(DPB_EINVAL, "cannot bind %u of %u variables", k, n);
     if (k * dtype_size(chal_dtype(mle->dtype)) > ctx->stage_bytes)
         return fail(DPB_EINVAL, "point too long");

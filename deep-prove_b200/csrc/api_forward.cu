@@ -7,12 +7,15 @@
 
 namespace dpb {
 
-// mapped page: [0] {findings, sequence number} of the last check, [8] set by a kernel that gave up waiting
+// mapped page: 8-byte words; 0 {findings, sequence number} of the last check, 1 set by a kernel that gave up waiting,
+// kSlotWord + i the check that holds slot i
+constexpr size_t kFwdPage = 1024;
+constexpr int kSlotWord = 8, kSlots = 64;
 static int fwd_init(dpb_ctx* ctx) {
     if (ctx->fwd_words) return DPB_OK;
     if (!ctx->fwd_host) {
-        DPB_CUDA(cudaHostAlloc(&ctx->fwd_host, 64, cudaHostAllocMapped));
-        memset(ctx->fwd_host, 0, 64);
+        DPB_CUDA(cudaHostAlloc(&ctx->fwd_host, kFwdPage, cudaHostAllocMapped));
+        memset(ctx->fwd_host, 0, kFwdPage);
         DPB_CUDA(cudaHostGetDevicePointer(&ctx->fwd_dev, ctx->fwd_host, 0));
     }
     unsigned int* w = nullptr;
@@ -28,7 +31,16 @@ static int fwd_init(dpb_ctx* ctx) {
 
 unsigned int* fwd_gave_up_word(dpb_ctx* ctx) { return (unsigned int*)ctx->fwd_dev + 2; }
 
-int fwd_check_begin(dpb_ctx* ctx, FwdCheck* out) {
+int fwd_slot_take(dpb_ctx* ctx) {
+    for (int i = 0; i < kSlots; i++)
+        if (!(ctx->fwd_slots >> i & 1)) {
+            ctx->fwd_slots |= 1ull << i;
+            return i;
+        }
+    return -1;
+}
+
+int fwd_check_begin(dpb_ctx* ctx, FwdCheck* out, int slot) {
     DPB_TRY(fwd_init(ctx));
     volatile unsigned int* gave_up = (volatile unsigned int*)ctx->fwd_host + 2;
     if (*gave_up) {
@@ -36,13 +48,13 @@ int fwd_check_begin(dpb_ctx* ctx, FwdCheck* out) {
         return fail(DPB_ETIMEOUT, "a kernel of an earlier forward call gave up waiting; that call's result is not valid");
     }
     out->words = ctx->fwd_words;
-    out->status = (unsigned long long*)ctx->fwd_dev;
+    out->status = (unsigned long long*)ctx->fwd_dev + (slot < 0 ? 0 : kSlotWord + slot);
     out->seq = ++ctx->fwd_seq;
     return DPB_OK;
 }
 
 int fwd_check_wait(dpb_ctx* ctx, const FwdCheck& c, unsigned int* found) {
-    const volatile uint64_t* status = (const volatile uint64_t*)ctx->fwd_host;
+    const volatile uint64_t* status = (const volatile uint64_t*)ctx->fwd_host + (c.status - (unsigned long long*)ctx->fwd_dev);
     const auto t0 = std::chrono::steady_clock::now();
     uint64_t spins = 0;
     for (;;) {
@@ -59,6 +71,18 @@ int fwd_check_wait(dpb_ctx* ctx, const FwdCheck& c, unsigned int* found) {
             if (dt > 120.0) return fail(DPB_ETIMEOUT, "waited %.1f s for a value check", dt);
         }
     }
+}
+
+int fwd_groups_verdict(const dpb_row_groups* g) {
+    if (g->slot >= 0) {
+        unsigned int found = 0;
+        DPB_TRY(fwd_check_wait(g->ctx, g->check, &found));
+        g->ctx->fwd_slots &= ~(1ull << g->slot);
+        g->slot = -1;
+        g->bad = found != 0;
+    }
+    if (g->bad) return fail(DPB_EINVAL, "a key lies outside 0..%llu", (unsigned long long)(g->n_keys - 1));
+    return DPB_OK;
 }
 
 int fwd_tensor(dpb_ctx* ctx, const int64_t* src, int on_device, uint64_t numel, const int64_t** dev, void** owned) {
@@ -172,8 +196,10 @@ static int groups_impl(dpb_ctx* ctx, const int64_t* keys, int on_device, dpb_row
         if (dense) DPB_CUDA(cudaMemsetAsync(counts, 0, (uint64_t)counters * 4, ctx->stream));
         return DPB_OK;
     }
-    FwdCheck check;
-    DPB_TRY(fwd_check_begin(ctx, &check));
+    const int slot = on_device ? fwd_slot_take(ctx) : -1;  // a host buffer is only read during the call: waited for here
+    g->slot = slot;
+    DPB_TRY(fwd_check_begin(ctx, &g->check, slot));
+    const FwdCheck check = g->check;
     const int64_t* dev = nullptr;
     void *owned = nullptr, *scratch = nullptr;
     DPB_TRY(fwd_tensor(ctx, keys, on_device, n, &dev, &owned));
@@ -198,12 +224,15 @@ static int groups_impl(dpb_ctx* ctx, const int64_t* keys, int on_device, dpb_row
             }
         }
     }
-    unsigned int found = 0;
-    if (rc == DPB_OK)
-        rc = e == cudaSuccess ? fwd_check_wait(ctx, check, &found) : fail(DPB_ECUDA, "sorting rows: %s", cudaGetErrorString(e));
+    if (rc == DPB_OK && e != cudaSuccess) rc = fail(DPB_ECUDA, "sorting rows: %s", cudaGetErrorString(e));
+    if (rc == DPB_OK && slot < 0) {
+        unsigned int found = 0;
+        rc = fwd_check_wait(ctx, check, &found);
+        g->bad = found != 0;
+        if (rc == DPB_OK) rc = fwd_groups_verdict(g);
+    }
     device_free(ctx, owned);
     device_free(ctx, scratch);
-    if (rc == DPB_OK && found) rc = fail(DPB_EINVAL, "a key lies outside 0..%llu", (unsigned long long)(g->n_keys - 1));
     return rc;
 }
 
@@ -225,6 +254,7 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
     a.keys = g->keys;
     a.rows = g->rows;
     a.n = g->n;
+    a.n_keys = g->n_keys;
     a.weights = weights ? weights->ptr : nullptr;
     a.width = width;
     a.per = per;
@@ -244,9 +274,9 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
             a.parts = parts;
             const uint32_t grid = key_blocks + (uint32_t)slices;
             if (weights)
-                key_sums_kernel<F, true><<<grid, kKeySumThreads, 0, ctx->stream>>>(a, g->n_keys, out_keys, key_blocks, scale, scaled);
+                key_sums_kernel<F, true><<<grid, kKeySumThreads, 0, ctx->stream>>>(a, out_keys, key_blocks, scale, scaled);
             else
-                key_sums_kernel<F, false><<<grid, kKeySumThreads, 0, ctx->stream>>>(a, g->n_keys, out_keys, key_blocks, scale, scaled);
+                key_sums_kernel<F, false><<<grid, kKeySumThreads, 0, ctx->stream>>>(a, out_keys, key_blocks, scale, scaled);
             if (slices > 1)
                 key_sums_join_kernel<F><<<(uint32_t)((slices * 32 + kKeySumThreads - 1) / kKeySumThreads), kKeySumThreads, 0, ctx->stream>>>(
                     a, slices, scale, scaled);
@@ -255,14 +285,14 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
     } else {
         rc = fwd_tensor(ctx, rows, rows_on_device, (a.n + per - 1) / per * width, &a.x, &owned);
         const uint64_t per_block = weights ? 2 * kRowSumThreads : kRowSumThreads, col_blocks = (width + per_block - 1) / per_block;
-        // slices of at least 16 rows, and as many as make one wave of resident blocks: the reduction at the end of a
+        // slices of at least 16 rows (8 without products), and as many as make one wave of resident blocks: the reduction at the end of a
         // block's sums, some hundred rows' worth of products, is then paid the fewest times
         int resident = 1;
         const cudaError_t oe = weights ? cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, row_products_kernel<F, true>, kRowSumThreads, 0)
                                        : cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, row_sums_kernel<F>, kRowSumThreads, 0);
         if (rc == DPB_OK && oe != cudaSuccess) rc = fail(DPB_ECUDA, "row sums: %s", cudaGetErrorString(oe));
         const uint64_t want = std::min<uint64_t>(65535, std::max<uint64_t>(1, (uint64_t)ctx->sm_count * std::max(resident, 1) / col_blocks));
-        a.slice = std::max<uint64_t>(16, (a.n + want - 1) / want);
+        a.slice = std::max<uint64_t>(weights ? 16 : 8, (a.n + want - 1) / want);
         const uint64_t slices = (a.n + a.slice - 1) / a.slice;
         if (rc == DPB_OK && slices > 1) rc = device_alloc(ctx, slices * 2 * width * sizeof(E), &parts);
         if (rc == DPB_OK) {
@@ -287,6 +317,7 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
     device_free(ctx, owned);
     device_free(ctx, parts);
     if (rc == DPB_OK && e != cudaSuccess) rc = fail(DPB_ECUDA, "row sums: %s", cudaGetErrorString(e));
+    if (rc == DPB_OK) rc = fwd_groups_verdict(g);
     if (rc != DPB_OK) {
         dpb_mle_free(m);
         return rc;
@@ -342,6 +373,8 @@ extern "C" uint64_t dpb_row_groups_len(const dpb_row_groups* g) { return g ? g->
 
 extern "C" void dpb_row_groups_free(dpb_row_groups* g) {
     if (!g) return;
+    // a check still under way publishes into its slot before any later one does, and under its own sequence number
+    if (g->slot >= 0) g->ctx->fwd_slots &= ~(1ull << g->slot);
     if (g->block) device_free(g->ctx, g->block);
     delete g;
 }
@@ -361,6 +394,7 @@ extern "C" int dpb_row_groups_sum(dpb_ctx* ctx, const dpb_row_groups* g, int fam
         if (weights->len < g->n)
             return fail(DPB_EINVAL, "%llu weights for %llu rows", (unsigned long long)weights->len, (unsigned long long)g->n);
     }
+    if (g->bad) return fwd_groups_verdict(g);
     if (pow2_ceil(g->n_keys) * pow2_ceil(width) > (1ull << 36)) return fail(DPB_EINVAL, "a result of more than 2^36 entries");
     const FwdDevice dev(ctx);
     DPB_CUDA(dev.err);

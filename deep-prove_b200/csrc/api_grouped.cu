@@ -82,17 +82,6 @@ static int product_impl(dpb_ctx* ctx, int dtype, const dpb_row_groups* g, const 
     cudaError_t e = cudaSuccess;
     unsigned int found = 0;
     if (rc == DPB_OK) {
-        const uint64_t cuts = n / per * ((w->k_blocks + 1) / 2), per_block = kCutThreads / 32;
-        const uint32_t blocks = (uint32_t)std::min<uint64_t>((cuts + per_block - 1) / per_block, (uint64_t)ctx->sm_count * 8);
-        const size_t smem = (w->n_experts + 1) * 4;
-        const int64_t half = 1ll << (x_bits - 1);
-        if (digits == 1)
-            cut_rows_kernel<1><<<blocks, kCutThreads, smem, ctx->stream>>>(dev, g->keys, g->places, g->offsets, n / per, per, w->n_experts, w->inner,
-                                                                           w->k_blocks, T, half, (int8_t*)planes, check);
-        else
-            cut_rows_kernel<2><<<blocks, kCutThreads, smem, ctx->stream>>>(dev, g->keys, g->places, g->offsets, n / per, per, w->n_experts, w->inner,
-                                                                           w->k_blocks, T, half, (int8_t*)planes, check);
-        e = cudaGetLastError();
         GroupedArgs a;
         memset(&a, 0, sizeof a);
         a.weights = w->planes;
@@ -112,7 +101,18 @@ static int product_impl(dpb_ctx* ctx, int dtype, const dpb_row_groups* g, const 
         splits = std::max<uint64_t>(splits, (w->k_blocks + kMaxSteps - 1) / kMaxSteps);
         a.blocks_per_split = (uint32_t)((w->k_blocks + splits - 1) / splits);
         a.splits = (w->k_blocks + a.blocks_per_split - 1) / a.blocks_per_split;
-        if (e == cudaSuccess && a.splits > 1) e = cudaMemsetAsync(a.out, 0, n * w->cols * 8, ctx->stream);
+        const uint64_t cuts = n / per * ((w->k_blocks + 1) / 2), per_block = kCutThreads / 32, clear = a.splits > 1 ? n * w->cols : 0;
+        const uint64_t for_cuts = (cuts + per_block - 1) / per_block, for_clear = (clear + 8 * kCutThreads - 1) / (8 * kCutThreads);
+        const uint32_t blocks = (uint32_t)std::min<uint64_t>(std::max(for_cuts, for_clear), (uint64_t)ctx->sm_count * 8);
+        const size_t smem = (w->n_experts + 1) * 4;
+        const int64_t half = 1ll << (x_bits - 1);
+        if (digits == 1)
+            cut_rows_kernel<1><<<blocks, kCutThreads, smem, ctx->stream>>>(dev, g->keys, g->places, g->offsets, n / per, per, w->n_experts, w->inner,
+                                                                           w->k_blocks, T, half, (int8_t*)planes, a.out, clear, check);
+        else
+            cut_rows_kernel<2><<<blocks, kCutThreads, smem, ctx->stream>>>(dev, g->keys, g->places, g->offsets, n / per, per, w->n_experts, w->inner,
+                                                                           w->k_blocks, T, half, (int8_t*)planes, a.out, clear, check);
+        e = cudaGetLastError();
         const uint32_t grid = (uint32_t)std::min<uint64_t>(max_tiles * w->col_tiles * a.splits, workers);
         if (e == cudaSuccess) {
             if (digits == 1) e = w->digits == 1 ? launch_rows<1, 1>(ctx, a, T, grid) : launch_rows<1, 2>(ctx, a, T, grid);
@@ -122,6 +122,7 @@ static int product_impl(dpb_ctx* ctx, int dtype, const dpb_row_groups* g, const 
     }
     device_free(ctx, owned);
     device_free(ctx, planes);
+    if (rc == DPB_OK) rc = fwd_groups_verdict(g);
     if (rc == DPB_OK && found) rc = fail(DPB_EINVAL, "a value of x does not fit %u bits", x_bits);
     if (rc != DPB_OK) {
         dpb_mle_free(m);
@@ -176,6 +177,7 @@ extern "C" int dpb_grouped_product(dpb_ctx* ctx, int family_dtype, const dpb_row
     if (!valid_dtype(family_dtype)) return fail(DPB_EINVAL, "unknown dtype %d", family_dtype);
     if (g->n_keys != w->n_experts)
         return fail(DPB_EINVAL, "rows routed to %llu experts, weights of %u", (unsigned long long)g->n_keys, w->n_experts);
+    if (g->bad) return fwd_groups_verdict(g);
     if (x_bits < 2 || x_bits > 15) return fail(DPB_EINVAL, "rows of %u bits (2..15)", x_bits);
     if (rows_per_token < 1 || g->n % rows_per_token)
         return fail(DPB_EINVAL, "%llu routed rows are not a multiple of %u per token", (unsigned long long)g->n, rows_per_token);

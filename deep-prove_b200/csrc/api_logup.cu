@@ -36,6 +36,7 @@ static int check_spec(dpb_ctx* ctx, const LogupSpec& p) {
     if (p.mult && (p.mult->len != len || is_gl(p.mult->dtype) != gl))
         return fail(DPB_EINVAL, "Multiplicities length was not equal to column evaluations length, multiplicities: %llu, columns: %llu",
                     (unsigned long long)p.mult->len, (unsigned long long)len);
+    if (!is_pow2(len)) return fail(DPB_EINVAL, "columns of %llu entries, not a power of two", (unsigned long long)len);
     if (len < 4) return fail(DPB_EINVAL, "columns need at least 4 entries, got %llu", (unsigned long long)len);
     return DPB_OK;
 }

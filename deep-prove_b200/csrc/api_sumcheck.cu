@@ -1439,6 +1439,10 @@ static int begin_general(dpb_ctx* ctx, uint32_t num_vars, dpb_mle* const* mles, 
             return fail(DPB_EINVAL, "table %u is null, foreign or of another field", j);
         }
         const uint32_t nv = log2u(m->len);
+        if (m->len != (1ull << nv)) {  // a tensor, or the owner of several tables
+            delete sc;
+            return fail(DPB_EINVAL, "table %u has %llu entries, not a power of two", j, (unsigned long long)m->len);
+        }
         if (nv < 1 || nv > num_vars) {
             delete sc;
             return fail(DPB_EINVAL, "table %u has %u variables, sumcheck has %u", j, nv, num_vars);

@@ -177,6 +177,7 @@ struct dpb_ctx {
     void* fwd_dev = nullptr;
     unsigned int* fwd_words = nullptr;
     unsigned int fwd_seq = 0;
+    uint64_t fwd_slots = 0;  // places in the mapped page that checks of row groups hold, a bit each
     // optional per-kernel timing log (dpb_profile_enable)
     bool profile = false;
     cudaEvent_t prof_ev[2] = {nullptr, nullptr};

@@ -3,20 +3,7 @@
 #pragma once
 #include "common.cuh"
 
-struct dpb_row_groups {
-    dpb_ctx* ctx = nullptr;
-    uint64_t n = 0, n_keys = 0;
-    void* block = nullptr;
-    uint32_t* keys = nullptr;     // the keys, ascending
-    uint32_t* rows = nullptr;     // the row at each place of that order
-    uint32_t* places = nullptr;   // the place of each row
-    uint32_t* offsets = nullptr;  // first place of every key (n_keys + 1 entries); null beyond kGroupOffsets keys
-};
-
 namespace dpb {
-
-constexpr uint32_t kGroupOffsets = 4095;  // with the end, one tile of the counting sort's scan
-
 enum FwdError : unsigned int { kFwdKeyRange = 1, kFwdValueRange = 2 };
 
 // How a kernel tells the host what it thinks of its input: the checking blocks or their findings into `words[0]`, the
@@ -29,6 +16,27 @@ struct FwdCheck {
     unsigned long long* status;  // mapped
     unsigned int seq;
 };
+}  // namespace dpb
+
+struct dpb_row_groups {
+    dpb_ctx* ctx = nullptr;
+    uint64_t n = 0, n_keys = 0;
+    // Keys on the device are checked there while the host goes on; the first call that uses the rows waits for the
+    // findings, behind its own launches.
+    mutable dpb::FwdCheck check = {};
+    mutable int slot = -1;     // the check's place in the mapped page, -1 once its findings are known
+    mutable bool bad = false;  // a key lies outside the range
+    void* block = nullptr;
+    uint32_t* keys = nullptr;     // the keys, ascending
+    uint32_t* rows = nullptr;     // the row at each place of that order
+    uint32_t* places = nullptr;   // the place of each row
+    uint32_t* offsets = nullptr;  // first place of every key (n_keys + 1 entries); null beyond kGroupOffsets keys
+};
+
+namespace dpb {
+
+constexpr uint32_t kGroupOffsets = 4095;  // with the end, one tile of the counting sort's scan
+
 // Called by every thread of each of the `blocks` checking blocks, once, after its checks; `found` is the thread's.
 __device__ __forceinline__ void fwd_check_done(const FwdCheck& c, unsigned int found, unsigned int blocks) {
     const unsigned int all = (__syncthreads_or((int)(found & kFwdKeyRange)) ? kFwdKeyRange : 0u) |
@@ -58,8 +66,12 @@ struct FwdDevice {
     }
 };
 
-// The next check of the context (api_forward.cu); DPB_ETIMEOUT when a kernel of an earlier call gave up waiting.
-int fwd_check_begin(dpb_ctx* ctx, FwdCheck* out);
+// The next check of the context (api_forward.cu); DPB_ETIMEOUT when a kernel of an earlier call gave up waiting.  With a
+// slot (fwd_slot_take) the findings stay readable until the slot is given back; without one, until the next check.
+int fwd_check_begin(dpb_ctx* ctx, FwdCheck* out, int slot = -1);
+int fwd_slot_take(dpb_ctx* ctx);  // -1: none is free
+// What the check of the rows' keys found, waiting for it if need be: DPB_EINVAL for a key outside the range.
+int fwd_groups_verdict(const dpb_row_groups* g);
 // Waits (bounded) for the check's findings.
 int fwd_check_wait(dpb_ctx* ctx, const FwdCheck& c, unsigned int* found);
 // The word in mapped memory a kernel that gives up waiting sets (device address).

@@ -254,8 +254,8 @@ __global__ void __launch_bounds__(kThreads)
 struct RowSumArgs {
     const uint32_t* keys;
     const uint32_t* rows;
-    uint64_t n;
-    uint64_t slice;  // rows per slice
+    uint64_t n, n_keys;  // a row's key is below n_keys; n_keys itself marks rows whose key was out of range: no sum
+    uint64_t slice;      // rows per slice
     const void* weights;
     const int64_t* x;
     uint64_t width;
@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kRowSumThreads, sizeof(typename F::E) == 32 ? 
                 const bool after = p0 + t + 1 == end && end < a.n && a.keys[end] == key;
 #pragma unroll
                 for (int q = 0; q < C; q++) {
-                    if (live[q]) {
+                    if (live[q] && key < a.n_keys) {
                         const uint64_t c = c0 + q;
                         E v = RowWords<F>::value(sum[q]);
                         if (any_wide) v = F::add(v, wide[q]);
@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(kRowSumThreads)
                 if (ends[i]) {
                     const uint32_t key = ends[i] - 1;
                     const bool after = p0 + i + 1 == end && end < a.n && a.keys[end] == key;
-                    if (live) {
+                    if (live && key < a.n_keys) {
                         const uint64_t slot = ((uint64_t)blockIdx.y * 2 + (before ? 0 : 1)) * a.width + c;
                         store_sum<F>(acc, before || after, scale, multiplier, before || after ? a.parts : a.out,
                                      before || after ? slot : (uint64_t)key * a.out_width + c);
@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(kRowSumThreads)
     const uint64_t begin = blockIdx.y * a.slice, end = begin + a.slice;
     if (end >= a.n) return;
     const uint32_t key = a.keys[end - 1];
-    if (a.keys[end] != key) return;                     // nothing goes on
+    if (a.keys[end] != key || key >= a.n_keys) return;  // nothing goes on
     if (begin > 0 && a.keys[begin - 1] == key) return;  // it began before
     const uint64_t last = (warp_first_at(a.keys, a.n, (uint64_t)key + 1) - 1) / a.slice;
     const uint64_t c = (uint64_t)blockIdx.x * kRowSumThreads + threadIdx.x;
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(kRowSumThreads)
 constexpr uint32_t kKeySumThreads = 256, kKeySumFew = 8, kKeySumSlice = 512;
 template <class F, bool W>
 __global__ void __launch_bounds__(kKeySumThreads)
-    key_sums_kernel(RowSumArgs a, uint64_t n_keys, uint64_t out_keys, uint32_t key_blocks, typename F::E multiplier, bool scale) {
+    key_sums_kernel(RowSumArgs a, uint64_t out_keys, uint32_t key_blocks, typename F::E multiplier, bool scale) {
     typedef typename F::E E;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto first_at = [&](uint64_t lo, uint64_t hi, uint64_t key) {  // first place in [lo, hi) whose key is not below
@@ -630,7 +630,7 @@ __global__ void __launch_bounds__(kKeySumThreads)
         __syncthreads();
         if (k >= out_keys) return;
         E v = F::zero();
-        if (k < n_keys && range[0] < range[1]) {
+        if (k < a.n_keys && range[0] < range[1]) {
             const uint64_t lo = first_at(range[0], range[1], k);
             uint32_t count = 0;
             uint32_t row[kKeySumFew];
@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(kKeySumThreads)
             while (lo > 0 && hi - lo <= kKeySumFew && a.keys[lo - 1] == key) lo--;
             is_long = hi - lo > kKeySumFew;
         }
-        if (is_long) starts[atomicAdd(&n_long, 1u)] = (uint32_t)(p - begin);
+        if (is_long && key < a.n_keys) starts[atomicAdd(&n_long, 1u)] = (uint32_t)(p - begin);
     }
     __syncthreads();
     const uint32_t count = n_long;
@@ -728,7 +728,7 @@ __global__ void __launch_bounds__(kKeySumThreads)
     const uint64_t begin = s * a.slice, end = begin + a.slice;
     if (end >= a.n) return;
     const uint32_t key = a.keys[end - 1];
-    if (a.keys[end] != key || (begin > 0 && a.keys[begin - 1] == key)) return;
+    if (a.keys[end] != key || key >= a.n_keys || (begin > 0 && a.keys[begin - 1] == key)) return;
     // a run of few rows is the key blocks' own
     uint64_t lo = end - 1;
     while (lo > begin && lo + kKeySumFew >= end && a.keys[lo - 1] == key) lo--;

@@ -118,11 +118,16 @@ template <int DIGITS>
 __global__ void __launch_bounds__(kCutThreads)
     cut_rows_kernel(const int64_t* __restrict__ x, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ places,
                     const uint32_t* __restrict__ offsets, uint64_t tokens, uint32_t per, uint32_t n_experts, uint64_t inner,
-                    uint32_t k_blocks, uint32_t T, int64_t half, int8_t* __restrict__ planes, FwdCheck check) {
+                    uint32_t k_blocks, uint32_t T, int64_t half, int8_t* __restrict__ planes,
+                    int64_t* __restrict__ clear, uint64_t n_clear, FwdCheck check) {
     extern __shared__ uint32_t tiles[];
     __shared__ __align__(16) uint8_t cut[kCutThreads / 32][DIGITS][kCutEntries];
     unsigned int found = 0;
     expert_tiles(offsets, n_experts, T, tiles);
+    // the output, when several work items will add to its entries (two per 16 bytes; it starts on a 256-byte boundary)
+    for (uint64_t i = (uint64_t)blockIdx.x * kCutThreads + threadIdx.x; i < n_clear / 2; i += (uint64_t)gridDim.x * kCutThreads)
+        ((longlong2*)clear)[i] = make_longlong2(0, 0);
+    if ((n_clear & 1) && blockIdx.x == 0 && threadIdx.x == 0) clear[n_clear - 1] = 0;
     __syncthreads();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t per_row = (k_blocks + 1) / 2;  // 256 entries = two stages
@@ -149,7 +154,9 @@ __global__ void __launch_bounds__(kCutThreads)
         if (digit < DIGITS && block < k_blocks) {
             const uint4 bytes = *(const uint4*)&cut[warp][digit][16 * piece];
             for (uint32_t j = 0; j < per; j++) {
-                const uint32_t p = places[token * per + j], e = keys[p], at = p - offsets[e], q = at / T;
+                const uint32_t p = places[token * per + j], e = keys[p];
+                if (e >= n_experts) continue;  // a key out of range: the call will be refused
+                const uint32_t at = p - offsets[e], q = at / T;
                 const uint64_t tile = (uint64_t)(tiles[e] + q) * k_blocks + block;
                 *(uint4*)(planes + (tile * DIGITS + digit) * (T * 128) + tile_piece(at - q * T, piece & 7)) = bytes;
             }

@@ -52,7 +52,8 @@ def embedding_lookup(ctx, table, vocab, width, tokens, multiplier=1, right_shift
 
 
 class RowGroups:
-    """dpb_row_groups: rows sorted by key (tokens, or the expert of every routed row)."""
+    """dpb_row_groups: rows sorted by key (tokens, or the expert of every routed row).  A key outside 0..n_keys-1 raises
+    here for keys on the host, in the first call that uses the rows for device_keys."""
 
     def __init__(self, ctx, keys, n_keys, device_keys=None):
         self.ctx, self.h = ctx, None

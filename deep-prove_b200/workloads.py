@@ -49,6 +49,9 @@ class TransformerShape:
     kv_heads: int = 0            # 0: as many as query heads; fewer: grouped-query attention (K and V shared by groups)
     glu: bool = False            # gated feed-forward (GeGLU / SwiGLU): two up projections and a GLU linking sumcheck
     rope: bool = False           # rotary positions on Q and K per block instead of one absolute-position layer
+    from_tokens: bool = False    # embeddings of a drawn token list, looked up on the backend, instead of a stand-in
+    experts: int = 0             # routed feed-forward layers: so many matrices (a power of two), 0 for dense ones
+    experts_per_token: int = 2
 
 
 @dataclass(frozen=True)
@@ -79,6 +82,8 @@ TINY = TransformerShape("tiny", layers=1, seq=24, d_model=48, heads=3, head_dim=
                         commit_chunk_log2=8, range_check_chunks=2)
 TINY_GLU_ROPE = TransformerShape("tiny-glu-rope-gqa", layers=1, seq=20, d_model=40, heads=4, head_dim=8, ffn=56,
                                  vocab=150, table_bits=8, commit_chunk_log2=8, kv_heads=2, glu=True, rope=True)
+TINY_EXPERTS = TransformerShape("tiny-experts", layers=1, seq=20, d_model=40, heads=4, head_dim=8, ffn=24, vocab=150,
+                                table_bits=8, commit_chunk_log2=8, kv_heads=2, rope=True, from_tokens=True, experts=4)
 TINY_MLP = MlpShape("tiny-mlp", widths=(48, 40, 10), table_bits=8, commit_chunk_log2=8)
 
 
@@ -148,6 +153,13 @@ def draw_tensor(rng, shape, spec):
     else:
         t = -rng.integers(0, big, size=shape, dtype=np.int64)
     return t
+
+
+class Resident:
+    """A tensor that an operator left on the backend, instead of an array to be uploaded."""
+
+    def __init__(self, handle, shape):
+        self.handle, self.shape = handle, tuple(shape)
 
 
 class PathTimer:
@@ -226,7 +238,8 @@ class PathWalk:
         both tensors are bound to (squeezed stand-ins for) the output claim's coordinates, the stacked axes (heads)
         share one point that gives the stacking coefficients, and the sumcheck runs over the contracted axis."""
         be, T, lg = self.be, self.T, ceil_log2
-        lhs_dev, rhs_dev = be.tensor(lhs), be.tensor(rhs)  # resident before the clock starts
+        # resident before the clock starts
+        lhs_dev, rhs_dev = lhs.handle if isinstance(lhs, Resident) else be.tensor(lhs), be.tensor(rhs)
         # the output claim's coordinates: stand-ins, drawn before the clock starts
         lp = [be.squeeze(T, lg(d)) if k != AX_CONTRACTED else None for d, k in zip(lhs.shape, lhs_kinds)]
         stacked = [p for p, k in zip(lp, lhs_kinds) if k == AX_STACKED]
@@ -359,6 +372,47 @@ class PathWalk:
             payload, point, finals = be.sumcheck(T, lg(pv), [one_hot, fixed], [(None, [0, 1])])
             self.rec.append(("embeddings", "embeddings", payload))
         be.free(fixed, one_hot)
+
+    def embeddings_of_tokens(self, wte, V, e, n):
+        """The forward lookup of n drawn tokens and the proof of its result's claim at a row and column point: the row
+        point's eq table summed by token takes the one-hot table's place, so that the sumcheck's sum is the embeddings'
+        value at the two points (transformer/embeddings.rs:395-445).  Returns the embeddings, resident."""
+        be, T, lg = self.be, self.T, ceil_log2
+        pv, pe = wte.shape
+        wte_tab = be.int_table(wte.reshape(-1))
+        self.committed.append(("wte", wte_tab, wte.size))
+        tokens = self.rng.integers(0, V, size=n, dtype=np.int64)
+        with self.timer("embedding_lookup"):
+            rows = be.embedding_lookup(wte_tab, V, e, pe, tokens)
+        row_point, col_point = be.squeeze(T, lg(n)), be.squeeze(T, lg(pe))
+        with self.timer("embeddings"):
+            by_token = be.row_sums(tokens, V, be.eq_table(row_point))
+            fixed = be.fix_low(wte_tab, col_point)
+            payload, point, finals = be.sumcheck(T, lg(pv), [by_token, fixed], [(None, [0, 1])])
+        claim = be.tensor_value(rows, (n, e), row_point, col_point)
+        self.rec.append(("embeddings", "embeddings", be.export([claim]) + payload))
+        be.free(fixed, by_token)
+        return Resident(rows, (n, e))
+
+    def experts(self, name, x, keys, weights, per):
+        """A routed layer: row i of the result is row i // per of x times the matrix keys[i] picks.  Forward by the grouped
+        product; its claim at a row and column point is the sum over (expert, inner) of the rows bound to the row point
+        inside each expert times the weights bound to the column point."""
+        be, T, lg = self.be, self.T, ceil_log2
+        g, k, c = weights.shape
+        self.commit_weight(name + ".w", weights.reshape(g * k, c))
+        x_dev, w_dev = be.tensor(x), be.tensor(weights)
+        with self.timer("grouped_product"):
+            groups, laid_out = be.row_groups(keys, g), be.expert_weights(w_dev, self.bits)
+            y = be.grouped_product(groups, x_dev, self.act_bits, laid_out, per)
+        row_point, col_point = be.squeeze(T, lg(len(keys))), be.squeeze(T, lg(c))
+        with self.timer("experts"):
+            lhs = be.group_sums(groups, be.eq_table(row_point), x_dev, per)
+            rhs = be.bind_columns(w_dev, weights.shape, col_point)
+            payload, point, finals = be.sumcheck(T, lg(g) + lg(k), [lhs, rhs], [(None, [0, 1])])
+        claim = be.tensor_value(y, (len(keys), c), row_point, col_point)
+        self.rec.append((name, "experts", be.export([claim]) + payload))
+        be.free(lhs, rhs, groups, laid_out, y, x_dev, w_dev)
 
     def positional(self, e):
         """Positional (absolute): fixed_positional * lt * column_eq over the embedding columns
@@ -502,12 +556,15 @@ def transformer_path(be, shape, seed=0, blocks=None, with_final=True, with_commi
     def gamma_table():
         return be.int_table(np.tile(np.pad(w.weights(e), (0, (1 << lg(e)) - e)), 1 << lg(s)))
 
-    wte = None
+    wte = embedded = None
     if with_final:
         pv, pe = 1 << lg(V), 1 << lg(e)
         wte = np.zeros((pv, pe), dtype=np.int64)
         wte[:V, :e] = w.weights((V, e))
-        w.embeddings(wte, V, e)
+        if shape.from_tokens:
+            embedded = w.embeddings_of_tokens(wte, V, e, s)
+        else:
+            w.embeddings(wte, V, e)
         if not shape.rope:
             w.positional(e)
 
@@ -519,7 +576,7 @@ def transformer_path(be, shape, seed=0, blocks=None, with_final=True, with_commi
         qkv_cols = (h + 2 * kv) * dh
         w_qkv = w.weights((e, qkv_cols))
         w.commit_weight(pre + "w_qkv", w_qkv)
-        w.einsum(pre + "qkv", x, (O, C), w_qkv, (C, O))
+        w.einsum(pre + "qkv", embedded if b == 0 and embedded else x, (O, C), w_qkv, (C, O))
         w.lookup_layer(pre + "qkv.requant", w.draw((s, qkv_cols), "requant"), "requant")
         if shape.rope:
             w.rope(pre + "rope_q", h, s, dh)
@@ -538,6 +595,17 @@ def transformer_path(be, shape, seed=0, blocks=None, with_final=True, with_commi
         w.einsum(pre + "out", w.small((s, h * dh)), (O, C), w_o, (C, O))
         w.same_poly(pre + "residual1", (1 << lg(s)) * (1 << lg(e)), 2)
         w.lookup_layer(pre + "norm2", w.draw((s, e), "norm"), "norm", VARIANT_NORMALISATION, gamma)
+        if shape.experts:
+            # a router's choice (drawn): different experts per token, some experts with few rows
+            per = shape.experts_per_token
+            keys = np.stack([w.rng.permutation(shape.experts)[:per] for _ in range(s)]).reshape(-1)
+            w.experts(pre + "ffn_up", x, keys, w.weights((shape.experts, e, f)), per)
+            w.lookup_layer(pre + "gelu", w.draw((s * per, f), "gelu"), "gelu")
+            w.experts(pre + "ffn_down", w.small((s * per, f)), keys, w.weights((shape.experts, f, e)), 1)
+            w.lookup_layer(pre + "ffn_down.requant", w.draw((s, e), "requant"), "requant")
+            w.same_poly(pre + "residual2", (1 << lg(s)) * (1 << lg(e)), 2)
+            be.free(gamma)
+            continue
         w_up = w.weights((e, f))
         w.commit_weight(pre + "w_up", w_up)
         w.einsum(pre + "ffn_up", x, (O, C), w_up, (C, O))
@@ -603,7 +671,9 @@ class GpuBackend:
     device; the transcript and the expression algebra run in the library's host code)."""
 
     def __init__(self, dpb, prover, ctx, field="fr", int_tables=True):
+        import importlib
         self.dpb, self.prover, self.ctx = dpb, prover, ctx
+        self.forward = importlib.import_module(dpb.__name__ + ".forward")
         # int_tables: integer tensors (weights, activations, fixed 0/1 tables) stay 32- or 64-bit integers on the
         # device instead of being converted to field elements at upload; every result is the same
         self.int_tables = int_tables
@@ -723,6 +793,45 @@ class GpuBackend:
         owner, tabs = self.ctx.einsum_fix_axes(self.fam, None, kinds, pts, device_tensor=tensor)
         tensor[0].free()
         return owner, tabs
+
+    # -- forward operators and what binds them
+    def embedding_lookup(self, table, vocab, width, stride, tokens):
+        return self.forward.embedding_lookup(self.ctx, table, vocab, width, tokens, row_stride=stride)
+
+    def row_groups(self, keys, n_keys):
+        return self.forward.RowGroups(self.ctx, keys, n_keys)
+
+    def group_sums(self, groups, weights, rows, per):
+        out = groups.sums(self.fam, weights=weights, device_rows=rows, rows_per_token=per)
+        weights.free()
+        return out
+
+    def row_sums(self, keys, n_keys, weights):
+        groups = self.row_groups(keys, n_keys)
+        out = groups.sums(self.fam, weights=weights)
+        weights.free()
+        groups.free()
+        return out
+
+    def expert_weights(self, w, bits):
+        return self.forward.ExpertWeights(self.ctx, None, bits, device_weights=w)
+
+    def grouped_product(self, groups, x, bits, weights, per):
+        return self.forward.grouped_product(self.ctx, groups, None, bits, weights, per, device_x=x, family_dtype=self.fam)
+
+    def bind_columns(self, w, shape, point):
+        """[expert, in, out] bound at the columns' point: one table over (expert, padded in)"""
+        owner, views = self.ctx.einsum_fix_axes(self.fam, None, (AX_STACKED, AX_CONTRACTED, AX_OUTER), [None, None, self._pt(point)],
+                                                device_tensor=w)
+        self.free(*views)
+        return owner
+
+    def tensor_value(self, tensor, shape, row_point, col_point):
+        owner, views = self.ctx.einsum_fix_axes(self.fam, None, (AX_OUTER, AX_OUTER), [self._pt(row_point), self._pt(col_point)],
+                                                device_tensor=tensor)
+        value = views[0].to_host().reshape(-1)
+        self.free(*views, owner)
+        return value
 
     def eq_table(self, point):
         return self.ctx.eq_table(self.fam, self._pt(point))

@@ -10,6 +10,7 @@ exports them, so equal protocol outputs give equal bytes.
 """
 import numpy as np
 
+from . import forward as fwd
 from . import oracle as orc
 
 
@@ -108,6 +109,43 @@ class OracleBackend:
 
     def fix_axes(self, tensor, kinds, points):
         return None, orc.mles_from_tensor(self.F, tensor, tuple(kinds), list(points))
+
+    # -- forward operators and what binds them (oracle/forward.py)
+    def embedding_lookup(self, table, vocab, width, stride, tokens):
+        p = orc.FR_MOD if self.F is orc.FrField else orc.GL_MOD
+        ints = np.array([v if v < p // 2 else v - p for v in self._ints(table)], dtype=np.int64)
+        return fwd.embedding_lookup(ints[:vocab * stride].reshape(vocab, stride)[:, :width], tokens)
+
+    def _ints(self, table):
+        vals = self.F.table_to_ints(table)
+        return [v[0] if isinstance(v, tuple) else int(v) for v in vals]
+
+    def row_groups(self, keys, n_keys):
+        return (np.asarray(keys), n_keys)
+
+    def group_sums(self, groups, weights, rows, per):
+        keys, n_keys = groups
+        w = orc.array_to_scalars(self.F, np.asarray(weights))
+        return orc.scalars_to_array(self.F, fwd.row_sums(self.F, keys, n_keys, w, rows, per))
+
+    def row_sums(self, keys, n_keys, weights):
+        w = orc.array_to_scalars(self.F, np.asarray(weights))
+        return orc.scalars_to_array(self.F, fwd.row_sums(self.F, keys, n_keys, w))
+
+    def expert_weights(self, w, bits):
+        return w
+
+    def grouped_product(self, groups, x, bits, weights, per):
+        return fwd.grouped_product(x, groups[0], weights, per)
+
+    def bind_columns(self, w, shape, point):
+        F = self.F
+        tabs = orc.mles_from_tensor(F, w, (orc.AXIS_STACKED, orc.AXIS_CONTRACTED, orc.AXIS_OUTER), [None, None, list(point)])
+        return np.concatenate([np.asarray(t) for t in tabs])
+
+    def tensor_value(self, tensor, shape, row_point, col_point):
+        tab = orc.mles_from_tensor(self.F, tensor, (orc.AXIS_OUTER, orc.AXIS_OUTER), [list(row_point), list(col_point)])[0]
+        return orc.array_to_scalars(self.F, np.asarray(tab))[0]
 
     def eq_table(self, point):
         return orc.eq_evals(self.F, list(point))

@@ -104,6 +104,20 @@ def test_lookup_refusals(dpb, ctx, fw):
     assert np.array_equal(read(got, shape), np.arange(16).reshape(2, 8))
 
 
+def test_a_tensor_is_no_table(dpb, ctx, fw):
+    """The unpadded result's handle is refused where a table's variables count, unless its length is a power of two."""
+    tab = ctx.upload_ints(np.arange(64), dpb.GL_I32)
+    tensor, shape = fw.embedding_lookup(ctx, tab, 8, 8, np.array([3, 1, 7]))
+    point = np.ones((2, 2), np.uint64)
+    terms = dpb.make_terms([(0, [0])], lambda c: dpb.one_bytes(dpb.GL_EXT))
+    for call in (lambda: ctx.sumcheck(5, [tensor], terms), lambda: ctx.fix_low(tensor, point), lambda: ctx.fix_high(tensor, point),
+                 lambda: ctx.logup(dpb.LOGUP_LOOKUP, [tensor], point[:1], point[:1])):
+        with pytest.raises(dpb.DpbError, match="power of two"):
+            call()
+    tensor, shape = fw.embedding_lookup(ctx, tab, 8, 8, np.array([3, 1]))
+    assert ctx.fix_low(tensor, point).len == 4
+
+
 # ------------------------------------------------------------------------------------------------ sums by key
 def random_weights(F, rng, n):
     t = F.random_ext_table(rng, n) if F is orc.GlField else F.random_table(rng, n)
@@ -204,6 +218,47 @@ def test_groups_refusals(dpb, ctx, fw):
         dpb.check(dpb.lib.dpb_row_groups_sum(ctx.h, g.h, dpb.FR, None, None, 0, 2, 1, 1, dpb.ctypes.byref(dpb.ctypes.c_void_p())))
     with pytest.raises(ValueError):
         g.sums(dpb.FR, rows=np.zeros((2, 4), np.int64))
+
+
+@pytest.mark.parametrize("n_keys", [4, 5, 2048])
+@pytest.mark.parametrize("n,bad", [(3, [2]), (3000, range(0, 3000, 7)), (700, range(600)), (6000, [5999]), (5000, range(5000))])
+def test_bad_device_keys(dpb, ctx, fw, n_keys, n, bad):
+    """Keys on the device are refused by the call that uses them, in every form, and nothing outside the result is
+    written: tables made before keep their entries."""
+    rng = np.random.default_rng(n)
+    keys = rng.integers(0, n_keys, size=n)
+    keys[list(bad)] = [n_keys, -1, 2**40][n % 3]
+    neighbours = [ctx.upload(rng.integers(0, 2**60, size=(4096, 4), dtype=np.uint64), dpb.FR) for _ in range(4)]
+    before = [t.to_host() for t in neighbours]
+    dev = ctx.upload_tensor_i64(keys)
+    w = ctx.upload(np.ones((pow2(n), 4), np.uint64), dpb.FR)
+    rows = np.ones((n, 3), np.int64)
+    for kw in (dict(weights=w), dict(), dict(rows=rows), dict(rows=rows, weights=w)):
+        g = fw.RowGroups(ctx, None, n_keys, device_keys=dev)
+        for _ in range(2):  # and again, once it is known
+            with pytest.raises(dpb.DpbError, match="key lies outside"):
+                g.sums(dpb.FR, **kw)
+        g.free()
+    if n_keys <= 5:
+        wt = fw.ExpertWeights(ctx, np.ones((n_keys, 3, 4), np.int64), 8)
+        g = fw.RowGroups(ctx, None, n_keys, device_keys=dev)
+        with pytest.raises(dpb.DpbError, match="key lies outside"):
+            fw.grouped_product(ctx, g, rows, 8, wt)
+    for t, b in zip(neighbours, before):
+        assert np.array_equal(t.to_host(), b)
+
+
+def test_many_unused_groups(dpb, ctx, fw):
+    """More handles whose check nobody waited for than the context has places for."""
+    keys = [ctx.upload_tensor_i64(np.array([i % 3, 0, 2])) for i in range(100)]
+    gs = [fw.RowGroups(ctx, None, 3, device_keys=k) for k in keys]
+    for i in (99, 0, 70, 63, 64):
+        got = gs[i].sums(dpb.GL_EXT).to_host()
+        assert got[:, 0].tolist() == np.bincount([i % 3, 0, 2], minlength=4).tolist()
+    for g in gs[::-1]:
+        g.free()
+    g = fw.RowGroups(ctx, None, 3, device_keys=keys[1])
+    assert g.sums(dpb.GL_EXT).to_host()[:, 0].tolist() == [1, 1, 1, 0]
 
 
 # ------------------------------------------------------------------------------------------------ grouped products
