@@ -38,8 +38,7 @@ static int weights_impl(dpb_ctx* ctx, const int64_t* src, int on_device, dpb_exp
     const int64_t* dev = nullptr;
     void* owned = nullptr;
     DPB_TRY(fwd_tensor(ctx, src, on_device, numel, &dev, &owned));
-    const uint64_t pieces = (uint64_t)w->n_experts * w->k_blocks * 8 * w->col_tiles * kTileCols;
-    const uint32_t blocks = (uint32_t)std::min<uint64_t>((pieces + kCutThreads - 1) / kCutThreads, (uint64_t)ctx->sm_count * 16);
+    const uint32_t blocks = (uint32_t)std::min<uint64_t>((uint64_t)w->n_experts * w->k_blocks * w->col_tiles, (uint64_t)ctx->sm_count * 4);
     const int64_t half = 1ll << (w->bits - 1);
     if (w->digits == 1)
         cut_weights_kernel<1><<<blocks, kCutThreads, 0, ctx->stream>>>(dev, w->n_experts, w->inner, w->cols, w->col_tiles, w->k_blocks,

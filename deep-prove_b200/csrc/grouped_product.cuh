@@ -36,54 +36,52 @@ constexpr uint32_t kMaxSteps = 256;  // stages per work item: 2^15 inner entries
 // 16-byte pieces of a row exchanged by xor with r mod 8.  One copy then brings a whole tile, with no tensor map.
 __device__ __forceinline__ uint32_t tile_piece(uint32_t row, uint32_t piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
 
-// 16 values -> 16-byte pieces of their digits; whether all lie in range
-template <int DIGITS>
-__device__ __forceinline__ bool cut_digits(const int64_t (&x)[16], int64_t half, uint4 (&out)[DIGITS]) {
-    uint32_t w[DIGITS][4];
-    bool ok = true;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        uint32_t d0 = 0, d1 = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int64_t v = x[4 * i + j];
-            ok = ok && v >= -half && v < half;
-            const int lo = (int)(int8_t)v;
-            d0 |= (uint32_t)(uint8_t)lo << (8 * j);
-            if (DIGITS == 2) d1 |= (uint32_t)(uint8_t)(((int)v - lo) >> 8) << (8 * j);
-        }
-        w[0][i] = d0;
-        if (DIGITS == 2) w[DIGITS - 1][i] = d1;
-    }
-#pragma unroll
-    for (int d = 0; d < DIGITS; d++) out[d] = make_uint4(w[d][0], w[d][1], w[d][2], w[d][3]);
-    return ok;
-}
-
-// Weights [expert][inner][cols] -> planes.  A thread takes 16 inner entries of one column: neighbouring threads read
-// neighbouring columns.  Made once per model.
 constexpr uint32_t kCutThreads = 256;
+// Weights [expert][inner][cols] -> planes, a tile of 128 columns by 128 inner entries at a time: neighbouring threads
+// read neighbouring columns, and the digits go through shared memory so that a tile is written as it lies.  Made once
+// per model.
 template <int DIGITS>
 __global__ void __launch_bounds__(kCutThreads)
     cut_weights_kernel(const int64_t* __restrict__ w, uint32_t n_experts, uint64_t inner, uint64_t cols, uint32_t col_tiles,
                        uint32_t k_blocks, int64_t half, int8_t* __restrict__ planes, FwdCheck check) {
+    __shared__ uint4 tile[DIGITS][kTileBytes / 16];
     unsigned int found = 0;
-    const uint64_t padded = (uint64_t)col_tiles * kTileCols, pieces = (uint64_t)k_blocks * 8;
-    const uint64_t total = n_experts * pieces * padded;
-    for (uint64_t t = (uint64_t)blockIdx.x * kCutThreads + threadIdx.x; t < total; t += (uint64_t)gridDim.x * kCutThreads) {
-        const uint64_t c = t % padded, q = t / padded, piece = q % pieces, e = q / pieces;
-        int64_t x[16];
+    const uint32_t col = threadIdx.x & 127, side = threadIdx.x >> 7;
+    const uint64_t total = (uint64_t)n_experts * col_tiles * k_blocks;
+    for (uint64_t t = blockIdx.x; t < total; t += gridDim.x) {
+        const uint64_t k0 = t % k_blocks * kTileK, ec = t / k_blocks, c = ec % col_tiles * kTileCols + col, e = ec / col_tiles;
+        const int64_t* src = w + (e * inner + k0) * cols + c;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const uint64_t k = piece * 16 + i;
-            x[i] = c < cols && k < inner ? w[(e * inner + k) * cols + c] : 0;
+        for (uint32_t q = 0; q < 4; q++) {
+            const uint32_t piece = 4 * side + q;
+            int64_t v[16];
+#pragma unroll
+            for (uint32_t i = 0; i < 16; i++) {
+                const uint32_t k = 16 * piece + i;
+                v[i] = c < cols && k0 + k < inner ? __ldcs((const long long*)src + (uint64_t)k * cols) : 0;
+            }
+            uint32_t d[DIGITS][4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                uint32_t d0 = 0, d1 = 0;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) {
+                    const int64_t x = v[4 * i + j];
+                    if (x < -half || x >= half) found = kFwdValueRange;
+                    const int lo = (int)(int8_t)x;
+                    d0 |= (uint32_t)(uint8_t)lo << (8 * j);
+                    d1 |= (uint32_t)(uint8_t)(((int)x - lo) >> 8) << (8 * j);
+                }
+                d[0][i] = d0;
+                if (DIGITS == 2) d[DIGITS - 1][i] = d1;
+            }
+#pragma unroll
+            for (int i = 0; i < DIGITS; i++) tile[i][tile_piece(col, piece) / 16] = make_uint4(d[i][0], d[i][1], d[i][2], d[i][3]);
         }
-        uint4 d[DIGITS];
-        if (!cut_digits<DIGITS>(x, half, d)) found = kFwdValueRange;
-        const uint64_t tile = (e * col_tiles + c / kTileCols) * k_blocks + piece / 8;
-#pragma unroll
-        for (int i = 0; i < DIGITS; i++)
-            *(uint4*)(planes + (tile * DIGITS + i) * kTileBytes + tile_piece(c % kTileCols, piece % 8)) = d[i];
+        __syncthreads();
+        uint4* out = (uint4*)(planes + t * DIGITS * kTileBytes);
+        for (uint32_t i = threadIdx.x; i < DIGITS * kTileBytes / 16; i += kCutThreads) __stcs(out + i, (&tile[0][0])[i]);
+        __syncthreads();
     }
     fwd_check_done(check, found, gridDim.x);
 }
