@@ -181,7 +181,7 @@ static int lookup_impl(dpb_ctx* ctx, const dpb_mle* table, uint64_t vocab, uint6
 
 static int groups_impl(dpb_ctx* ctx, const int64_t* keys, int on_device, dpb_row_groups* g) {
     const uint32_t n = (uint32_t)g->n, n_keys = (uint32_t)g->n_keys;
-    const bool small = n <= kSmallSort, dense = n_keys <= kGroupOffsets;
+    const bool few = n_keys <= kFewKeys && n > kSmallSort && n <= kFewSort, small = n <= kSmallSort || few, dense = n_keys <= kGroupOffsets;
     const uint32_t counters = n_keys + 1, tiles = (counters + kCountTile - 1) / kCountTile;
     // one block: [keys | rows | places | offsets or counters]
     auto up = [](uint64_t words) { return (words + 63) & ~63ull; };
@@ -205,7 +205,10 @@ static int groups_impl(dpb_ctx* ctx, const int64_t* keys, int on_device, dpb_row
     DPB_TRY(fwd_tensor(ctx, keys, on_device, n, &dev, &owned));
     int rc = DPB_OK;
     cudaError_t e = cudaSuccess;
-    if (small) {
+    if (few) {
+        groups_few_kernel<<<1, kFewThreads, (n_keys + 1) * 128, ctx->stream>>>(dev, n, n_keys, g->keys, g->rows, g->places, g->offsets, check);
+        e = cudaGetLastError();
+    } else if (small) {
         const uint32_t probes = n + (dense ? n_keys + 1 : 0), per_block = kSmallSortThreads / 8;
         groups_small_kernel<<<(probes + per_block - 1) / per_block, kSmallSortThreads, ((n + 31) & ~31u) * 4, ctx->stream>>>(
             dev, n, n_keys, g->keys, g->rows, g->places, g->offsets, check);
@@ -217,10 +220,11 @@ static int groups_impl(dpb_ctx* ctx, const int64_t* keys, int on_device, dpb_row
             e = cudaMemsetAsync(counts, 0, (uint64_t)counters * 4, ctx->stream);
             if (e == cudaSuccess) {
                 groups_count_kernel<<<grid_for(ctx, n), kThreads, 0, ctx->stream>>>(dev, n, n_keys, counts, rank, check);
-                groups_scan_kernel<<<tiles, 1024, 0, ctx->stream>>>(counts, counters, tile_sums);
-                groups_scatter_kernel<<<grid_for(ctx, n), kThreads, 0, ctx->stream>>>(dev, n, n_keys, counts, tile_sums, tiles, rank,
-                                                                                      g->keys, g->rows);
-                e = cudaGetLastError();
+                e = launch_early(ctx->stream, tiles, 1024, 0, groups_scan_kernel, counts, counters, tile_sums);
+                if (e == cudaSuccess)
+                    e = launch_early(ctx->stream, grid_for(ctx, n), kThreads, 0, groups_scatter_kernel, dev, n, n_keys, counts, tile_sums, tiles,
+                                     rank, g->keys, g->rows);
+                if (e == cudaSuccess) e = cudaGetLastError();
             }
         }
     }
@@ -273,14 +277,11 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
         if (rc == DPB_OK) {
             a.parts = parts;
             const uint32_t grid = key_blocks + (uint32_t)slices;
-            if (weights)
-                key_sums_kernel<F, true><<<grid, kKeySumThreads, 0, ctx->stream>>>(a, out_keys, key_blocks, scale, scaled);
-            else
-                key_sums_kernel<F, false><<<grid, kKeySumThreads, 0, ctx->stream>>>(a, out_keys, key_blocks, scale, scaled);
-            if (slices > 1)
-                key_sums_join_kernel<F><<<(uint32_t)((slices * 32 + kKeySumThreads - 1) / kKeySumThreads), kKeySumThreads, 0, ctx->stream>>>(
-                    a, slices, scale, scaled);
-            e = cudaGetLastError();
+            e = launch_early(ctx->stream, grid, kKeySumThreads, 0, weights ? key_sums_kernel<F, true> : key_sums_kernel<F, false>, a, out_keys,
+                             key_blocks, scale, scaled);
+            if (slices > 1 && e == cudaSuccess)
+                e = launch_early(ctx->stream, (uint32_t)((slices * 32 + kKeySumThreads - 1) / kKeySumThreads), kKeySumThreads, 0,
+                                 key_sums_join_kernel<F>, a, slices, scale, scaled);
         }
     } else {
         rc = fwd_tensor(ctx, rows, rows_on_device, (a.n + per - 1) / per * width, &a.x, &owned);
@@ -300,15 +301,13 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
             e = cudaMemsetAsync(m->ptr, 0, m->len * sizeof(E), ctx->stream);  // keys without rows, and the padding
             if (e == cudaSuccess && a.n) {
                 const dim3 grid((uint32_t)col_blocks, (uint32_t)slices);
-                if (weights && (width & 1) == 0 && ((uintptr_t)a.x & 15) == 0)
-                    row_products_kernel<F, true><<<grid, kRowSumThreads, 0, ctx->stream>>>(a, scale, scaled);
-                else if (weights) row_products_kernel<F, false><<<grid, kRowSumThreads, 0, ctx->stream>>>(a, scale, scaled);
-                else row_sums_kernel<F><<<grid, kRowSumThreads, 0, ctx->stream>>>(a, scale, scaled);
-                if (slices > 1) {
+                auto kernel = !weights ? row_sums_kernel<F>
+                              : (width & 1) == 0 && ((uintptr_t)a.x & 15) == 0 ? row_products_kernel<F, true> : row_products_kernel<F, false>;
+                e = launch_early(ctx->stream, grid, kRowSumThreads, 0, kernel, a, scale, scaled);
+                if (slices > 1 && e == cudaSuccess) {
                     const dim3 join((uint32_t)((width + kRowSumThreads - 1) / kRowSumThreads), (uint32_t)slices);
-                    row_sums_join_kernel<F><<<join, kRowSumThreads, 0, ctx->stream>>>(a, scale, scaled);
+                    e = launch_early(ctx->stream, join, kRowSumThreads, 0, row_sums_join_kernel<F>, a, scale, scaled);
                 }
-                e = cudaGetLastError();
             }
         }
     }

@@ -13,8 +13,7 @@ static cudaError_t launch_product(dpb_ctx* ctx, const GroupedArgs& a, uint32_t b
     const uint32_t smem = GroupedShape<XD, WD, T>::smem(a.n_experts);
     cudaError_t e = cudaFuncSetAttribute(grouped_product_kernel<XD, WD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    grouped_product_kernel<XD, WD, T><<<blocks, kGroupedThreads, smem, ctx->stream>>>(a);
-    return cudaGetLastError();
+    return launch_early(ctx->stream, blocks, kGroupedThreads, smem, grouped_product_kernel<XD, WD, T>, a);
 }
 template <int XD, int WD>
 static cudaError_t launch_rows(dpb_ctx* ctx, const GroupedArgs& a, uint32_t rows, uint32_t blocks) {
@@ -71,8 +70,8 @@ static int product_impl(dpb_ctx* ctx, int dtype, const dpb_row_groups* g, const 
     // Rows per tile.  An instruction takes as long for 16 rows as for 128 (about 70 clocks; 85 for 160), so a tile should
     // hold what an expert gets: fewer, fuller tiles read the weights less often.  Small tiles leave room for more stages
     // (few rows: bound by the weights' way from HBM) and, up to 64 rows of two digits, for a second accumulator.
-    // Measured: 52 rows per expert 24.9 us with 64, 25.9 with 128; 128 rows 61 us with 128, 67 with 64 or 160; 2048 rows
-    // 1.95 ms with 160, 2.20 with 128, 3.45 with 64.
+    // Measured: 52 rows per expert 24.9 us with 64, 25.9 with 128; 128 rows 68 us the call with 128, 73 with 80, 72 with 96;
+    // 2048 rows 1.95 ms with 160, 2.04 with 128, 3.4 with 64.
     const uint64_t used = std::min<uint64_t>(w->n_experts, n), average = (n + used - 1) / used;
     const uint32_t T = average <= 8 ? 16 : average <= 16 ? 32 : average <= 64 ? 64 : average < 320 ? 128 : 160;
     const uint64_t max_tiles = n / T + used;  // every expert's last tile may be partly filled
@@ -100,18 +99,20 @@ static int product_impl(dpb_ctx* ctx, int dtype, const dpb_row_groups* g, const 
         splits = std::max<uint64_t>(splits, (w->k_blocks + kMaxSteps - 1) / kMaxSteps);
         a.blocks_per_split = (uint32_t)((w->k_blocks + splits - 1) / splits);
         a.splits = (w->k_blocks + a.blocks_per_split - 1) / a.blocks_per_split;
+        // items, and an item's number plus a grid, are 32-bit numbers
+        if (max_tiles * w->col_tiles * a.splits >= (1ull << 32) - 4096) {
+            device_free(ctx, owned);
+            device_free(ctx, planes);
+            dpb_mle_free(m);
+            return fail(DPB_EINVAL, "%llu work items", (unsigned long long)(max_tiles * w->col_tiles * a.splits));
+        }
         const uint64_t cuts = n / per * ((w->k_blocks + 1) / 2), per_block = kCutThreads / 32, clear = a.splits > 1 ? n * w->cols : 0;
         const uint64_t for_cuts = (cuts + per_block - 1) / per_block, for_clear = (clear + 8 * kCutThreads - 1) / (8 * kCutThreads);
         const uint32_t blocks = (uint32_t)std::min<uint64_t>(std::max(for_cuts, for_clear), (uint64_t)ctx->sm_count * 8);
         const size_t smem = (w->n_experts + 1) * 4;
         const int64_t half = 1ll << (x_bits - 1);
-        if (digits == 1)
-            cut_rows_kernel<1><<<blocks, kCutThreads, smem, ctx->stream>>>(dev, g->keys, g->places, g->offsets, n / per, per, w->n_experts, w->inner,
-                                                                           w->k_blocks, T, half, (int8_t*)planes, a.out, clear, check);
-        else
-            cut_rows_kernel<2><<<blocks, kCutThreads, smem, ctx->stream>>>(dev, g->keys, g->places, g->offsets, n / per, per, w->n_experts, w->inner,
-                                                                           w->k_blocks, T, half, (int8_t*)planes, a.out, clear, check);
-        e = cudaGetLastError();
+        e = launch_early(ctx->stream, blocks, kCutThreads, smem, digits == 1 ? cut_rows_kernel<1> : cut_rows_kernel<2>, dev, g->keys, g->places,
+                         g->offsets, n / per, per, w->n_experts, w->inner, w->k_blocks, T, half, (int8_t*)planes, a.out, clear, check);
         const uint32_t grid = (uint32_t)std::min<uint64_t>(max_tiles * w->col_tiles * a.splits, workers);
         if (e == cudaSuccess) {
             if (digits == 1) e = w->digits == 1 ? launch_rows<1, 1>(ctx, a, T, grid) : launch_rows<1, 2>(ctx, a, T, grid);

@@ -35,7 +35,7 @@ struct dpb_row_groups {
 
 namespace dpb {
 
-constexpr uint32_t kGroupOffsets = 4095;  // with the end, one tile of the counting sort's scan
+constexpr uint32_t kGroupOffsets = 1024;  // what grouped products take; with the end, one tile of the counting sort's scan
 
 // Called by every thread of each of the `blocks` checking blocks, once, after its checks; `found` is the thread's.
 __device__ __forceinline__ void fwd_check_done(const FwdCheck& c, unsigned int found, unsigned int blocks) {
@@ -51,6 +51,27 @@ __device__ __forceinline__ void fwd_check_done(const FwdCheck& c, unsigned int f
         c.words[1] = 0;
     }
     *(volatile unsigned long long*)c.status = ((unsigned long long)c.seq << 32) | verdict;
+}
+
+// A kernel launched with launch_early may start while the stream's previous kernel runs, once all of that kernel's
+// blocks have called let_next_start (or ended); what that kernel, or any before it, writes may be read after
+// wait_for_previous, which waits for its end.  Such a kernel marks no pointer to that data __restrict__ and reads it with
+// no __ldg: loads of data that is constant for a whole kernel may be moved up past the wait.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <class... Params, class... Args>
+cudaError_t launch_early(cudaStream_t stream, dim3 blocks, uint32_t threads, size_t smem, void (*kernel)(Params...), Args... args) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim = blocks;
+    c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = stream;
+    cudaLaunchAttribute at = {};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, Params(args)...);
 }
 
 // Restores the caller's current device (the context's own may be another).

@@ -11,10 +11,10 @@
 // N: a warp's lanes then hold neighbouring columns of one output row, which is stored as whole 256-byte runs without a
 // transposition, and a tile of few rows (a single token) wastes nothing.
 //
-// What bounds it.  Many rows: the instruction, at two per 8-bit pair's worth of 16-bit work; 16384 routed rows of 4096 by
-// 8 matrices of 4096 x 11008 take 1.95 ms, 5.9e12 digit operations at 3.0 P/s against 3.3 P/s (twice the measured bf16
-// rate), with the power cap at work.  Two blocks sharing a tile (cta_group::2) brought less through L2 but took 2.02 ms.
-// One token through two experts: the weights' 180 MB from HBM, 37 us against 28.
+// What bounds it.  Many rows: the instruction.  16384 routed rows of 4096 by 8 matrices of 4096 x 11008 take 1.95 ms:
+// 5.9e12 digit operations at 3.0e15/s, where twice the measured bf16 rate is 3.3e15/s, with the power cap at work.  (Two
+// blocks sharing a tile by cta_group::2 bring less through L2 but took 2.02 ms.)  One token through two experts: the
+// weights' 180 MB from HBM, 36 us against 28.
 #pragma once
 #include "forward.cuh"
 
@@ -87,13 +87,13 @@ __global__ void __launch_bounds__(kCutThreads)
 }
 
 // first tile of every expert: tiles[e] = sum of ceil(rows / T) over the experts before e
-__device__ __forceinline__ void expert_tiles(const uint32_t* __restrict__ offsets, uint32_t n_experts, uint32_t T,
+__device__ __forceinline__ void expert_tiles(const uint32_t* offsets, uint32_t n_experts, uint32_t T,
                                              uint32_t* tiles /* shared, n_experts + 1 */) {
     if (threadIdx.x < 32) {
         uint32_t carry = 0;
         for (uint32_t e0 = 0; e0 < n_experts; e0 += 32) {
             const uint32_t e = e0 + threadIdx.x;
-            const uint32_t n = e < n_experts ? (offsets[e + 1] - offsets[e] + T - 1) / T : 0;
+            const uint32_t n = e < n_experts ? (__ldcg(offsets + e + 1) - __ldcg(offsets + e) + T - 1) / T : 0;
             uint32_t incl = n;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
@@ -114,13 +114,13 @@ __device__ __forceinline__ void expert_tiles(const uint32_t* __restrict__ offset
 constexpr uint32_t kCutEntries = 256;
 template <int DIGITS>
 __global__ void __launch_bounds__(kCutThreads)
-    cut_rows_kernel(const int64_t* __restrict__ x, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ places,
-                    const uint32_t* __restrict__ offsets, uint64_t tokens, uint32_t per, uint32_t n_experts, uint64_t inner,
-                    uint32_t k_blocks, uint32_t T, int64_t half, int8_t* __restrict__ planes,
-                    int64_t* __restrict__ clear, uint64_t n_clear, FwdCheck check) {
+    cut_rows_kernel(const int64_t* x, const uint32_t* keys, const uint32_t* places, const uint32_t* offsets, uint64_t tokens, uint32_t per, uint32_t n_experts, uint64_t inner,
+                    uint32_t k_blocks, uint32_t T, int64_t half, int8_t* planes, int64_t* clear, uint64_t n_clear, FwdCheck check) {
     extern __shared__ uint32_t tiles[];
     __shared__ __align__(16) uint8_t cut[kCutThreads / 32][DIGITS][kCutEntries];
     unsigned int found = 0;
+    wait_for_previous();
+    let_next_start();  // the product's kernel, not before the rows' order is there: it sets itself up and fetches weights
     expert_tiles(offsets, n_experts, T, tiles);
     // the output, when several work items will add to its entries (two per 16 bytes; it starts on a 256-byte boundary)
     for (uint64_t i = (uint64_t)blockIdx.x * kCutThreads + threadIdx.x; i < n_clear / 2; i += (uint64_t)gridDim.x * kCutThreads)
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kCutThreads)
 #pragma unroll
         for (uint32_t i = 0; i < kCutEntries / 32; i++) {
             const uint64_t k = k0 + 32 * i + lane;
-            v[i] = k < inner ? __ldg((const long long*)src + k) : 0;
+            v[i] = k < inner ? src[k] : 0;
         }
 #pragma unroll
         for (uint32_t i = 0; i < kCutEntries / 32; i++) {
@@ -219,13 +219,11 @@ __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint3
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-// 16 columns of the warp's 32 lanes
-__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(addr));
+// 8 columns of the warp's 32 lanes
+__device__ __forceinline__ void tmem_load8(uint32_t addr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
 }
 
 // ------------------------------------------------------------------------------------------------ the product
@@ -253,15 +251,16 @@ struct GroupedShape {
     static constexpr uint32_t smem(uint32_t n_experts) { return kStages * kStageBytes + 1024 + (n_experts + 1) * 4; }
 };
 
-// The eight warps that move a finished tile: warp w reads the accumulators' lanes 32 (w mod 4) .. + 31, that is 32
-// columns, and of the rows the sixteens w / 4, w / 4 + 2, ...  Accumulators wait for this when there is room for one
-// tile's only, so it is kept short: the rows' places in the output are read before the tile is finished (tile_rows), and
-// a sixteen's accumulators are on their way while the last one's results are stored.
-constexpr uint32_t kStoreWarps = 8, kGroupedThreads = 32 * (kStoreWarps + 2);
+// The sixteen warps that move a finished tile: warp w reads the accumulators' lanes 32 (w mod 4) .. + 31, that is 32
+// columns, and of the rows the eights w / 4, w / 4 + 4, ...  There is room for one large tile's accumulators only, so
+// they are turned into results in registers first and given back to the next tile's products, and stored after that
+// (512 rows routed to 8 experts: 61 us when they were given back between the stores); the rows' places in the output are
+// read before the tile is finished.
+constexpr uint32_t kStoreWarps = 16, kGroupedThreads = 32 * (kStoreWarps + 2);
 template <int T>
 struct TileRows {
     uint32_t row[(T + 31) / 32];  // lane l: rows l, l + 32, ... of the tile
-    __device__ __forceinline__ void load(const uint32_t* __restrict__ rows, uint32_t lo, int valid) {
+    __device__ __forceinline__ void load(const uint32_t* rows, uint32_t lo, int valid) {
 #pragma unroll
         for (int i = 0; i < (T + 31) / 32; i++) {
             const int j = 32 * i + (threadIdx.x & 31);
@@ -272,37 +271,37 @@ struct TileRows {
 // accumulators -> 64-bit results; `release` is called when the warp has read its accumulators
 template <int ACC, int T, class Release>
 __device__ __forceinline__ void store_tile(const GroupedArgs& a, uint32_t acc, const TileRows<T>& rows, int valid, uint64_t c,
-                                           uint32_t half, Release release) {
-    constexpr int kChunks = (T + 31) / 32;
-    uint32_t r[2][ACC][16];
-    const int mine = (valid - 16 * (int)half + 31) / 32;  // sixteens of this warp with a row in them
-    auto read = [&](int i) {
+                                           uint32_t quarter, Release release) {
+    constexpr int kEights = (T + 31) / 32;
+    int64_t y[kEights][8];
 #pragma unroll
-        for (int d = 0; d < ACC; d++) tmem_load16(acc + d * T + 32 * i + 16 * half, r[i & 1][d]);
-    };
-    auto done_reading = [&]() {
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        release();
-    };
-    if (mine > 0) read(0);
-    else done_reading();
+    for (int i = 0; i < kEights; i++) {
+        if (32 * i + 8 * (int)quarter >= valid) break;
+        uint32_t r[ACC][8];
 #pragma unroll
-    for (int i = 0; i < kChunks; i++) {
-        if (i >= mine) break;
+        for (int d = 0; d < ACC; d++) tmem_load8(acc + d * T + 32 * i + 8 * quarter, r[d]);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (i + 1 < kChunks && i + 1 < mine) read(i + 1);
-        else done_reading();
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const uint32_t row = __shfl_sync(0xffffffffu, rows.row[i], 16 * half + j);
-            int64_t y = (int32_t)r[i & 1][0][j];
+        for (int j = 0; j < 8; j++) {
+            y[i][j] = (int32_t)r[0][j];
 #pragma unroll
-            for (int d = 1; d < ACC; d++) y += (int64_t)(int32_t)r[i & 1][d][j] << (8 * d);
-            if (c < a.cols && 32 * i + 16 * (int)half + j < valid) {
+            for (int d = 1; d < ACC; d++) y[i][j] += (int64_t)(int32_t)r[d][j] << (8 * d);
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncwarp();
+    release();
+#pragma unroll
+    for (int i = 0; i < kEights; i++) {
+        const int j0 = 32 * i + 8 * (int)quarter;
+        if (j0 >= valid) break;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t row = __shfl_sync(0xffffffffu, rows.row[i], 8 * quarter + j);
+            if (c < a.cols && j0 + j < valid) {
                 int64_t* o = a.out + (uint64_t)row * a.cols + c;
-                if (a.splits > 1) atomicAdd((unsigned long long*)o, (unsigned long long)y);
-                else __stcs((long long*)o, (long long)y);
+                if (a.splits > 1) atomicAdd((unsigned long long*)o, (unsigned long long)y[i][j]);
+                else __stcs((long long*)o, (long long)y[i][j]);
             }
         }
     }
@@ -318,7 +317,7 @@ __device__ __forceinline__ void gave_up_wait(unsigned int* word) {
     __syncthreads();
 }
 
-// Ten warps: 0-7 move finished accumulators to the output, 8 brings the operands, 9 issues the products.  One block per
+// Eighteen warps: 0-15 move finished accumulators to the output, 16 brings the operands, 17 issues the products.  One block per
 // SM walks the work items blockIdx.x, + gridDim.x, ...; items of one expert are ordered with the row tiles fastest, so
 // that the blocks at work at one time share the weights' and rows' tiles in L2.
 template <int XD, int WD, int T>
@@ -359,20 +358,18 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_product_kernel(Gro
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_slot;
-    const uint64_t per_tile = (uint64_t)a.col_tiles * a.splits, items = tiles[a.n_experts] * per_tile;
+    const uint32_t per_tile = a.col_tiles * a.splits, items = tiles[a.n_experts] * per_tile;  // below 2^32 (the host's rule)
 
     // the item's expert (found by walking on from the last item's), its row tile, column tile and stages
     struct Item {
         uint32_t expert, row_tile, col_tile, first, last;
     };
-    auto item_at = [&](uint64_t i, uint32_t& e) {
+    auto item_at = [&](uint32_t i, uint32_t& e) {
         while (i >= tiles[e + 1] * per_tile) e++;
-        const uint32_t mine = tiles[e + 1] - tiles[e];
-        const uint64_t j = i - tiles[e] * per_tile;
+        const uint32_t mine = tiles[e + 1] - tiles[e], j = i - tiles[e] * per_tile, q = j / mine;
         Item it;
         it.expert = e;
-        it.row_tile = (uint32_t)(j % mine);
-        const uint32_t q = (uint32_t)(j / mine);
+        it.row_tile = j - q * mine;
         it.col_tile = q % a.col_tiles;
         it.first = q / a.col_tiles * a.blocks_per_split;
         it.last = it.first + a.blocks_per_split < a.k_blocks ? it.first + a.blocks_per_split : a.k_blocks;
@@ -382,15 +379,34 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_product_kernel(Gro
     uint32_t e = 0;
     if (warp == kStoreWarps && lane == 0) {
         uint32_t stage = 0, phase = 0;
-        for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {
+        auto weights_of = [&](const Item& it) {
+            return a.weights + ((uint64_t)(it.expert * a.col_tiles + it.col_tile) * a.k_blocks) * (WD * kTileBytes);
+        };
+        auto rows_of = [&](const Item& it) { return a.x + ((uint64_t)(tiles[it.expert] + it.row_tile) * a.k_blocks) * (XD * T * 128); };
+        // The rows' digits may still be in the making: the first item's first stages get their weights before that is over
+        uint32_t ahead = 0;
+        if (blockIdx.x < items) {
+            const Item it = item_at(blockIdx.x, e);
+            const int8_t* w = weights_of(it);
+            ahead = it.last - it.first < S::kStages ? it.last - it.first : S::kStages;
+            for (uint32_t s = 0; s < ahead; s++) {
+                bar_expect(full(s), S::kStageBytes);
+                bulk_load(ring + s * S::kStageBytes, w + (uint64_t)(it.first + s) * (WD * kTileBytes), WD * kTileBytes, full(s));
+            }
+        }
+        wait_for_previous();
+        for (uint32_t i = blockIdx.x; i < items; i += gridDim.x) {
             const Item it = item_at(i, e);
-            const int8_t* w = a.weights + ((uint64_t)(e * a.col_tiles + it.col_tile) * a.k_blocks) * (WD * kTileBytes);
-            const int8_t* x = a.x + ((uint64_t)(tiles[e] + it.row_tile) * a.k_blocks) * (XD * T * 128);
+            const int8_t *w = weights_of(it), *x = rows_of(it);
             for (uint32_t k = it.first; k < it.last; k++) {
                 if (!bar_wait(empty(stage), phase ^ 1, &gave_up)) goto done;
                 const uint32_t dst = ring + stage * S::kStageBytes;
-                bar_expect(full(stage), S::kStageBytes);
-                bulk_load(dst, w + (uint64_t)k * (WD * kTileBytes), WD * kTileBytes, full(stage));
+                if (ahead) {
+                    ahead--;
+                } else {
+                    bar_expect(full(stage), S::kStageBytes);
+                    bulk_load(dst, w + (uint64_t)k * (WD * kTileBytes), WD * kTileBytes, full(stage));
+                }
                 bulk_load(dst + WD * kTileBytes, x + (uint64_t)k * (XD * T * 128), XD * T * 128, full(stage));
                 if (++stage == S::kStages) {
                     stage = 0;
@@ -410,7 +426,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_product_kernel(Gro
         // D = S32, A and B = signed 8 bits, both K-major
         constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(T >> 3) << 17) | ((kTileCols >> 4) << 24);
         uint32_t stage = 0, phase = 0, buf = 0, buf_phase = 0;
-        for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {
+        for (uint32_t i = blockIdx.x; i < items; i += gridDim.x) {
             const Item it = item_at(i, e);
             if (!bar_wait(acc_empty(buf), buf_phase ^ 1, &gave_up)) goto done;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -443,8 +459,9 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_product_kernel(Gro
             }
         }
     } else if (warp < kStoreWarps) {
+        wait_for_previous();  // which may be clearing the output
         uint32_t buf = 0, buf_phase = 0;
-        for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {
+        for (uint32_t i = blockIdx.x; i < items; i += gridDim.x) {
             const Item it = item_at(i, e);
             const uint32_t lo = a.offsets[e] + it.row_tile * T, end = a.offsets[e + 1];
             const int valid = end - lo < T ? (int)(end - lo) : T;
