@@ -154,7 +154,13 @@ static int lookup_impl(dpb_ctx* ctx, const dpb_mle* table, uint64_t vocab, uint6
     const bool vec = a.out_width % V == 0 && stride % V == 0 && ((uintptr_t)table->ptr & 15) == 0 && vocab * stride <= table->len;
     const uint64_t steps = a.out_rows * ((a.out_width + (vec ? V : 1) - 1) / (vec ? V : 1));
     const uint32_t blocks = (uint32_t)std::min<uint64_t>((steps + kLookupThreads - 1) / kLookupThreads, (uint64_t)ctx->sm_count * 4);
-    const bool index32 = steps + 2ull * kLookupFlight * blocks * kLookupThreads < (1ull << 32);
+    const bool index32 = steps + 2ull * kLookupFlight * blocks * kLookupThreads < (1ull << 31);
+    // with l = ceil(log2 d) and m = floor(2^(31 + l) / d) + 1, w m / 2^(31 + l) lies less than 1 / d above w / d
+    const uint64_t per_row = a.out_width / (vec ? V : 1), l = log2u(per_row);
+    if (index32) {
+        a.div_mul = (uint32_t)((1ull << (31 + l)) / per_row + 1);
+        a.div_shift = (uint32_t)(31 + l);
+    }
     a.check_blocks = check_all ? 0 : (uint32_t)std::min<uint64_t>(blocks, (n + 8 * kLookupThreads - 1) / (8 * kLookupThreads));
     if (i32) {
         if (vec) launch_lookup<int32_t, 4>(ctx, a, check_all, index32, blocks);

@@ -44,8 +44,10 @@ __device__ __forceinline__ void fwd_check_done(const FwdCheck& c, unsigned int f
     if (threadIdx.x != 0) return;
     unsigned int verdict = all;
     if (blocks > 1) {
-        if (all) atomicOr(c.words, all);
-        __threadfence();
+        if (all) {
+            atomicOr(c.words, all);
+            __threadfence();  // before the ticket; with nothing found there is nothing to order, and results need not land
+        }
         if (atomicAdd(c.words + 1, 1u) != blocks - 1) return;
         verdict = atomicExch(c.words, 0u);
         c.words[1] = 0;

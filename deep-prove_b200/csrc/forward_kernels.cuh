@@ -17,6 +17,7 @@ struct LookupArgs {
     uint32_t shift;
     uint64_t out_rows, out_width;  // what is written: n x width, or the padded sizes
     int64_t* out;
+    uint32_t div_mul, div_shift;  // 32-bit steps: w / per_row = (w * div_mul) >> div_shift for w below 2^31
     uint32_t check_blocks;  // blocks that check the tokens; 0: every block, and the products as well
     FwdCheck check;
 };
@@ -35,7 +36,7 @@ __device__ __forceinline__ int64_t lookup_scale(const LookupArgs& a, int64_t x, 
 }
 
 // T: the table's integers; V: entries per step (1 or 16 bytes' worth on the narrower side).  I: the index type; 32 bits
-// wherever they suffice, since finding a step's row takes a division.  kLookupFlight steps per thread are under way
+// wherever they suffice, since finding a step's row takes a division (by a multiplication then).  kLookupFlight steps per thread are under way
 // together: tokens, then table entries, then results; steps of neighbouring threads are neighbours, and a thread's own
 // lie a grid apart (next to each other they fill fewer blocks of a short call: 8 us instead of 5).  16384 rows of 4096
 // entries of 8 bytes take 168 us: 1.07 GB, 4.3 TB/s of it from and to HBM and the rest rows that several tokens share.
@@ -57,8 +58,8 @@ __global__ void __launch_bounds__(kLookupThreads, sizeof(I) == 4 ? 4 : 2) embedd
         T x[kLookupFlight][V];
 #pragma unroll
         for (int f = 0; f < kLookupFlight; f++) {
-            const I w = w0 + f * step;  // 32 bits: total + 2 kLookupFlight step stays below 2^32 (the host's rule)
-            const I i = w / per_row;
+            const I w = w0 + f * step;  // 32 bits: total + 2 kLookupFlight step stays below 2^31 (the host's rule)
+            const I i = sizeof(I) == 4 ? (I)(((uint64_t)w * a.div_mul) >> a.div_shift) : w / per_row;
             row[f] = i;
             col[f] = (uint64_t)(w - i * per_row) * V;
             tok[f] = w < total && row[f] < a.n && col[f] < a.width ? (uint64_t)__ldg((const long long*)a.tokens + i) : ~0ull - 1;
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__(kLookupThreads, sizeof(I) == 4 ? 4 : 2) embedd
                     if (over) found |= kFwdValueRange;
                 }
             }
-            int64_t* o = a.out + row[f] * a.out_width + col[f];
+            int64_t* o = a.out + (uint64_t)(w0 + f * step) * V;  // rows follow one another: V divides the width written
             if constexpr (V == 1) {
                 *o = y[0];
             } else {
