@@ -299,7 +299,7 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
                                        : cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, row_sums_kernel<F>, kRowSumThreads, 0);
         if (rc == DPB_OK && oe != cudaSuccess) rc = fail(DPB_ECUDA, "row sums: %s", cudaGetErrorString(oe));
         const uint64_t want = std::min<uint64_t>(65535, std::max<uint64_t>(1, (uint64_t)ctx->sm_count * std::max(resident, 1) / col_blocks));
-        a.slice = std::max<uint64_t>(weights ? 16 : 8, (a.n + want - 1) / want);
+        a.slice = std::min<uint64_t>(kRowSumMaxSlice, std::max<uint64_t>(weights ? 16 : 8, (a.n + want - 1) / want));
         const uint64_t slices = (a.n + a.slice - 1) / a.slice;
         if (rc == DPB_OK && slices > 1) rc = device_alloc(ctx, slices * 2 * width * sizeof(E), &parts);
         if (rc == DPB_OK) {

@@ -364,6 +364,7 @@ struct RowSumArgs {
 // between the weights' and entries' way through shared memory (57 % of its wavefronts) and the instructions' issue (59 %).
 // What an entry has above 16 bits, as quantised activations do not, takes a field product.
 constexpr uint32_t kExactRows = 64;
+constexpr uint64_t kRowSumMaxSlice = 49152;  // rows per slice: 2^47 times as many stays below 2^63
 // an integer below 2^31 in magnitude as a double, by its place next to 2^52
 __device__ __forceinline__ double exact_double(int32_t x) {
     return __hiloint2double(0x43300000, x ^ (int32_t)0x80000000) - 4503601774854144.0;  // 2^52 + 2^31

@@ -12,7 +12,7 @@
  * Everything is exact: integers, or field elements in the layouts of dpb.h.
  *
  * Conventions are those of dpb.h.  Work is queued on the context's stream (dpb_stream); device inputs must be ready on
- * that stream, and results are ready on it.  Calls that check values on the device wait for that check before they
+ * that stream and stay as they are until it has passed the call, and results are ready on it.  Calls that check values on the device wait for that check before they
  * return, so they cannot be made inside a stream capture; their results may still be in the making.
  */
 #ifndef DPB_FORWARD_H

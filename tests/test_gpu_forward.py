@@ -189,6 +189,25 @@ def test_row_sums_full_range(dpb, ctx, fw, F, weights):
     check_sums(dpb, ctx, fw, F, keys, 2, weights, rows, m=-2**63)
 
 
+def test_row_sums_of_a_long_run(dpb, ctx, fw):
+    """One key with 70000 rows that all name the same wide row, entries and words of the weights at their largest: more
+    than 2^63 in a word's sum, unless the run is cut."""
+    n, width = 70000, 160000
+    limbs = np.array([2**64 - 1, 2**64 - 1, 2**64 - 1, 0x2fffffffffffffff], dtype=np.uint64)
+    table = np.zeros((1 << 17, 4), np.uint64)
+    table[:n] = limbs
+    weights = ctx.upload(table, dpb.FR)
+    x = np.full((1, width), -32768)
+    x[0, 1::2] = 32767
+    g = fw.RowGroups(ctx, np.zeros(n, np.int64), 1)
+    got = g.sums(dpb.FR, weights=weights, rows=x, rows_per_token=n).to_host(n=width)
+    w = sum(int(v) << (64 * i) for i, v in enumerate(limbs))
+    for c in (0, 1, width - 2, width - 1):
+        want = w * n * int(x[0, c]) % orc.FR_MOD
+        assert sum(int(v) << (64 * i) for i, v in enumerate(got[c])) == want
+    assert (got[0::2] == got[0]).all() and (got[1::2] == got[1]).all()
+
+
 @pytest.mark.parametrize("F", FIELDS)
 def test_no_rows_at_all(dpb, ctx, fw, F):
     g = fw.RowGroups(ctx, np.zeros(0, np.int64), 5)
