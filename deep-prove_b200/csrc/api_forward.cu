@@ -304,7 +304,10 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
         if (rc == DPB_OK && slices > 1) rc = device_alloc(ctx, slices * 2 * width * sizeof(E), &parts);
         if (rc == DPB_OK) {
             a.parts = parts;
-            e = cudaMemsetAsync(m->ptr, 0, m->len * sizeof(E), ctx->stream);  // keys without rows, and the padding
+            // keys without rows, and the padding: by the kernel where the keys' places are kept, which saves a launch
+            a.offsets = a.n ? g->offsets : nullptr;
+            a.out_keys = out_keys;
+            if (!a.offsets) e = cudaMemsetAsync(m->ptr, 0, m->len * sizeof(E), ctx->stream);
             if (e == cudaSuccess && a.n) {
                 const dim3 grid((uint32_t)col_blocks, (uint32_t)slices);
                 auto kernel = !weights ? row_sums_kernel<F>

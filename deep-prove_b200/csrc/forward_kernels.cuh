@@ -354,7 +354,19 @@ struct RowSumArgs {
     uint64_t out_width;
     void* out;
     void* parts;  // [slice][2][width]
+    const uint32_t* offsets;  // first places of the keys, where the kernel writes the zeros of the result; null: the host does
+    uint64_t out_keys;
 };
+
+// The result's entries that no sum goes to: rows of keys without rows, and the padding.  Every block takes some keys.
+template <class F>
+__device__ __forceinline__ void clear_unsummed(const RowSumArgs& a) {
+    if (!a.offsets) return;
+    for (uint64_t k = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x; k < a.out_keys; k += (uint64_t)gridDim.x * gridDim.y) {
+        const bool empty = k >= a.n_keys || a.offsets[k] == a.offsets[k + 1];
+        for (uint64_t c = (empty ? 0 : a.width) + threadIdx.x; c < a.out_width; c += blockDim.x) F::store(a.out, k * a.out_width + c, F::zero());
+    }
+}
 
 // An unreduced sum of (weight) * (integer) products.  A weight's 32-bit words and an entry of up to 16 bits are exact in
 // a double, a product is at most 2^47 and kExactRows of them stay within 2^53: the sums run as one fused multiply-add per
@@ -446,9 +458,9 @@ __device__ __noinline__ typename F::E add_high(typename F::E v, const typename F
 constexpr uint32_t kRowSumThreads = 128, kRowSumBatch = 64, kRowSumFlight = 8;
 
 // With weights: two columns per thread (a weight read from shared memory then serves two products).  The entries come
-// through a per-thread ring in shared memory, kRingAhead groups of four rows ahead of the products, so that loads are
-// under way all the time.
-constexpr uint32_t kRowRing = 4, kRingAhead = kRowRing - 1, kProductBatch = 128;
+// through a per-thread ring in shared memory, kRingAhead groups of eight rows ahead of the products, so that loads are
+// under way all the time (groups of four, three ahead: 64.5 us where these take 61.5).
+constexpr uint32_t kRowRing = 2, kRingAhead = kRowRing - 1, kProductBatch = 128, kGroup = 8;
 template <int BYTES>
 __device__ __forceinline__ void ring_load(void* dst, const void* src) {
     if constexpr (BYTES == 16)
@@ -464,8 +476,9 @@ __global__ void __launch_bounds__(kRowSumThreads, sizeof(typename F::E) == 32 ? 
     constexpr int C = 2, N = RowWords<F>::N;
     let_next_start();
     wait_for_previous();
+    clear_unsummed<F>(a);
     __shared__ __align__(16) double wsh[kProductBatch + 1][N];  // the last weight is zero
-    __shared__ longlong2 ring[kRowRing][4][kRowSumThreads];
+    __shared__ longlong2 ring[kRowRing][kGroup][kRowSumThreads];
     __shared__ const int64_t* from[kProductBatch];
     __shared__ uint32_t keys[kProductBatch];
     __shared__ uint32_t ends[kProductBatch / 32];  // a bit per row: the key's run ends here
@@ -513,11 +526,11 @@ __global__ void __launch_bounds__(kRowSumThreads, sizeof(typename F::E) == 32 ? 
         }
         __syncthreads();
         auto issue = [&](uint32_t g) {
-            if (4 * g < m) {
+            if (kGroup * g < m) {
                 longlong2* dst = &ring[g % kRowRing][0][tid];
 #pragma unroll
-                for (uint32_t u = 0; u < 4; u++) {  // rows past the batch's last repeat that one
-                    const int64_t* src = from[4 * g + u] + c_load;
+                for (uint32_t u = 0; u < kGroup; u++) {  // rows past the batch's last repeat that one
+                    const int64_t* src = from[kGroup * g + u] + c_load;
                     if (PAIRS) {
                         ring_load<16>(dst + u * kRowSumThreads, src);
                     } else {
@@ -537,7 +550,7 @@ __global__ void __launch_bounds__(kRowSumThreads, sizeof(typename F::E) == 32 ? 
             uint32_t h = s >> 5, rest = ends[h] >> (s & 31) << (s & 31);
             while (!rest && ++h < kProductBatch / 32) rest = ends[h];
             const uint32_t t = rest ? 32 * h + __ffs(rest) - 1 : m - 1;  // the run's last row here
-            for (uint32_t g = s >> 2; g <= t >> 2; g++) {
+            for (uint32_t g = s / kGroup; g <= t / kGroup; g++) {
                 if (g == next) {
                     asm volatile("cp.async.wait_group %0;" ::"n"(kRingAhead - 1) : "memory");
                     issue(g + kRingAhead);  // into the group before this one, whose products are done
@@ -546,8 +559,8 @@ __global__ void __launch_bounds__(kRowSumThreads, sizeof(typename F::E) == 32 ? 
                 bool more = false;  // an entry has more than 16 bits
                 const longlong2* x4 = &ring[g % kRowRing][0][tid];
 #pragma unroll
-                for (uint32_t u = 0; u < 4; u++) {
-                    const uint32_t i = 4 * g + u;
+                for (uint32_t u = 0; u < kGroup; u++) {
+                    const uint32_t i = kGroup * g + u;
                     const double* w = wsh[i >= s && i <= t ? i : kProductBatch];  // other runs' rows: times 0
                     const longlong2 x2 = x4[u * kRowSumThreads];
 #pragma unroll
@@ -561,15 +574,15 @@ __global__ void __launch_bounds__(kRowSumThreads, sizeof(typename F::E) == 32 ? 
                 }
                 if (more) {
 #pragma unroll 1
-                    for (uint32_t i = max(s, 4 * g); i <= min(t, 4 * g + 3); i++) {
+                    for (uint32_t i = max(s, kGroup * g); i <= min(t, kGroup * g + kGroup - 1); i++) {
                         const E w = F::load(a.weights, F::kChalDtype, a.rows[p0 + i]);
-                        const longlong2 x2 = x4[(i & 3) * kRowSumThreads];
+                        const longlong2 x2 = x4[i % kGroup * kRowSumThreads];
                         wide[0] = add_high<F>(wide[0], w, x2.x);
                         wide[1] = add_high<F>(wide[1], w, x2.y);
                     }
                     any_wide = true;
                 }
-                if (g % (kExactRows / 4) == kExactRows / 4 - 1) drain();
+                if (g % (kExactRows / kGroup) == kExactRows / kGroup - 1) drain();
             }
             drain();
             if (rest) {
@@ -615,6 +628,7 @@ __global__ void __launch_bounds__(kRowSumThreads)
     typedef typename F::E E;
     let_next_start();
     wait_for_previous();
+    clear_unsummed<F>(a);
     __shared__ uint64_t at[kRowSumBatch];
     __shared__ uint32_t ends[kRowSumBatch];
     const uint64_t c = (uint64_t)blockIdx.x * kRowSumThreads + threadIdx.x;
