@@ -614,9 +614,20 @@ __global__ void __launch_bounds__(kRowSumThreads, sizeof(typename F::E) == 32 ? 
     }
 }
 
+// an integer as a field element: from its two words where it fits 64 bits
+template <class F>
+__device__ __forceinline__ typename F::E field_from_int(__int128 v);
+template <>
+__device__ __forceinline__ Fr field_from_int<FrFam>(__int128 v) {
+    return v == (__int128)(int64_t)v ? fr_from_int_rows((int64_t)v) : field_from_i128<FrFam>(v);
+}
+template <>
+__device__ __forceinline__ Gl2 field_from_int<GlFam>(__int128 v) {
+    return v == (__int128)(int64_t)v ? gl2_from_base(GlFam::base_from_int((int64_t)v)) : field_from_i128<GlFam>(v);
+}
 template <class F>
 __device__ __noinline__ void store_sum(__int128 sum, bool part, bool scale, const typename F::E& multiplier, void* out, uint64_t i) {
-    typename F::E v = field_from_i128<F>(sum);
+    typename F::E v = field_from_int<F>(sum);
     if (scale && !part) v = F::mul(v, multiplier);
     F::store(out, i, v);
 }
