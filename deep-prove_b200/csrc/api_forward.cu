@@ -294,11 +294,8 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
         const uint64_t per_block = weights ? 2 * kRowSumThreads : kRowSumThreads, col_blocks = (width + per_block - 1) / per_block;
         // slices of at least 16 rows (8 without products), and as many as make one wave of resident blocks: the reduction at the end of a
         // block's sums, some hundred rows' worth of products, is then paid the fewest times
-        int resident = 1;
-        const cudaError_t oe = weights ? cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, row_products_kernel<F, true>, kRowSumThreads, 0)
-                                       : cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, row_sums_kernel<F>, kRowSumThreads, 0);
-        if (rc == DPB_OK && oe != cudaSuccess) rc = fail(DPB_ECUDA, "row sums: %s", cudaGetErrorString(oe));
-        const uint64_t want = std::min<uint64_t>(65535, std::max<uint64_t>(1, (uint64_t)ctx->sm_count * std::max(resident, 1) / col_blocks));
+        const uint64_t resident = weights ? kProductBlocks<F> : 8;
+        const uint64_t want = std::min<uint64_t>(65535, std::max<uint64_t>(1, (uint64_t)ctx->sm_count * resident / col_blocks));
         a.slice = std::min<uint64_t>(kRowSumMaxSlice, std::max<uint64_t>(weights ? 16 : 8, (a.n + want - 1) / want));
         const uint64_t slices = (a.n + a.slice - 1) / a.slice;
         if (rc == DPB_OK && slices > 1) rc = device_alloc(ctx, slices * 2 * width * sizeof(E), &parts);
@@ -309,7 +306,10 @@ static int sum_impl(dpb_ctx* ctx, const dpb_row_groups* g, const dpb_mle* weight
             a.out_keys = out_keys;
             if (!a.offsets) e = cudaMemsetAsync(m->ptr, 0, m->len * sizeof(E), ctx->stream);
             if (e == cudaSuccess && a.n) {
-                const dim3 grid((uint32_t)col_blocks, (uint32_t)slices);
+                // more blocks where the zeros would be many for the slices' own: 16 entries per thread, up to four per SM
+                const uint64_t for_zeros = std::min<uint64_t>(m->len / (16 * kRowSumThreads), (uint64_t)ctx->sm_count * 4);
+                const uint64_t rows_of_blocks = a.offsets ? std::max(slices, (for_zeros + col_blocks - 1) / col_blocks) : slices;
+                const dim3 grid((uint32_t)col_blocks, (uint32_t)std::min<uint64_t>(rows_of_blocks, 65535));
                 auto kernel = !weights ? row_sums_kernel<F>
                               : (width & 1) == 0 && ((uintptr_t)a.x & 15) == 0 ? row_products_kernel<F, true> : row_products_kernel<F, false>;
                 e = launch_early(ctx->stream, grid, kRowSumThreads, 0, kernel, a, scale, scaled);

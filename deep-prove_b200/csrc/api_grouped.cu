@@ -1,5 +1,6 @@
 // C ABI: integer matrix products grouped by expert (include/dpb_forward.h).
 #include <algorithm>
+#include <atomic>
 
 #include "../../include/dpb_forward.h"
 #include "grouped_product.cuh"
@@ -11,8 +12,15 @@ static uint32_t digits_of(uint32_t bits) { return bits <= 8 ? 1 : 2; }
 template <int XD, int WD, int T>
 static cudaError_t launch_product(dpb_ctx* ctx, const GroupedArgs& a, uint32_t blocks) {
     const uint32_t smem = GroupedShape<XD, WD, T>::smem(a.n_experts);
-    cudaError_t e = cudaFuncSetAttribute(grouped_product_kernel<XD, WD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
+    // once per device: the most that any number of experts takes
+    static std::atomic<uint64_t> allowed{0};
+    const uint64_t bit = ctx->device < 64 ? 1ull << ctx->device : 0;
+    if (!(allowed.load(std::memory_order_relaxed) & bit) || !bit) {
+        const cudaError_t e = cudaFuncSetAttribute(grouped_product_kernel<XD, WD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)GroupedShape<XD, WD, T>::smem(1024));
+        if (e != cudaSuccess) return e;
+        allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
     return launch_early(ctx->stream, blocks, kGroupedThreads, smem, grouped_product_kernel<XD, WD, T>, a);
 }
 template <int XD, int WD>
