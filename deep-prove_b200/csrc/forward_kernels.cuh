@@ -375,7 +375,7 @@ __device__ __forceinline__ void clear_unsummed(const RowSumArgs& a) {
 // a double, a product is at most 2^47 and kExactRows of them stay within 2^53: the sums run as one fused multiply-add per
 // word on the 64-bit floating-point pipe, exactly, and move to signed 64-bit integers every kExactRows rows.  Wide integer
 // multiply-adds run at half a double's rate, and came with as many moves: 8192 rows of 4096 over BN254 took 88 us in a
-// chain of carries, 76 us in one 64-bit accumulator per word, and take 63 us this way.  What bounds it then is shared
+// chain of carries, 76 us in one 64-bit accumulator per word, and take 59 us this way.  What bounds it then is shared
 // between the weights' and entries' way through shared memory (57 % of its wavefronts) and the instructions' issue (59 %).
 // What an entry has above 16 bits, as quantised activations do not, takes a field product.
 constexpr uint32_t kExactRows = 64;
