@@ -115,12 +115,6 @@ struct GlFam {
         r.c1 = __shfl_down_sync(0xffffffffu, (unsigned long long)v.c1, off);
         return r;
     }
-    __device__ __forceinline__ static E shfl_up(const E& v, int off) {
-        E r;
-        r.c0 = __shfl_up_sync(0xffffffffu, (unsigned long long)v.c0, off);
-        r.c1 = __shfl_up_sync(0xffffffffu, (unsigned long long)v.c1, off);
-        return r;
-    }
 #endif
 };
 
@@ -178,13 +172,6 @@ struct FrFam {
 #pragma unroll
         for (int j = 0; j < 4; j++)
             r.l[j] = __shfl_down_sync(0xffffffffu, (unsigned long long)v.l[j], off);
-        return r;
-    }
-    __device__ __forceinline__ static E shfl_up(const E& v, int off) {
-        E r;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            r.l[j] = __shfl_up_sync(0xffffffffu, (unsigned long long)v.l[j], off);
         return r;
     }
 #endif
