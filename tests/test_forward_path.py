@@ -154,3 +154,45 @@ def test_two_contexts_and_another_stream(dpb, ctx):
         other.sync()
     finally:
         other.close()
+
+
+@pytest.mark.gpu
+def test_two_threads_with_a_context_each(dpb, ctx):
+    """Two host threads work at the same time, each on a context of its own: products and sums of both share the GPU."""
+    import threading
+    fw = importlib.import_module("deep_prove_b200.forward")
+    failures = []
+
+    def work(seed):
+        try:
+            c = dpb.Context(0)
+            rng = np.random.default_rng(seed)
+            W = rng.integers(-2048, 2048, size=(5, 300, 260))
+            laid_out = fw.ExpertWeights(c, W, 12)
+            for _ in range(15):
+                n = int(rng.integers(1, 400))
+                keys, x = rng.integers(0, 5, size=n), rng.integers(-8192, 8192, size=(n, 300))
+                g = fw.RowGroups(c, None, 5, device_keys=c.upload_tensor_i64(keys))
+                y, shape = fw.grouped_product(c, g, x, 14, laid_out)
+                s = g.sums(dpb.GL_EXT, rows=x)
+                want = np.zeros((8, 512), dtype=object)
+                for k in range(5):
+                    want[k, :300] = x[keys == k].sum(axis=0)
+                got = s.to_host().reshape(8, 512, 2)
+                if not np.array_equal(y.to_host(n=n * 260).reshape(shape), ofw.grouped_product(x, keys, W)):
+                    failures.append((seed, "product"))
+                if (got[:, :, 0].astype(object) != want % orc.GL_MOD).any() or got[:, :, 1].any():
+                    failures.append((seed, "sums"))
+                for h in (y, s, g):
+                    h.free()
+            laid_out.free()
+            c.close()
+        except Exception as e:  # a thread's exception must not pass unseen
+            failures.append((seed, repr(e)))
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in (1, 2, 3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
