@@ -404,6 +404,7 @@ extern "C" int dpb_row_groups_sum(dpb_ctx* ctx, const dpb_row_groups* g, int fam
     }
     if (g->bad) return fwd_groups_verdict(g);
     if (pow2_ceil(g->n_keys) * pow2_ceil(width) > (1ull << 36)) return fail(DPB_EINVAL, "a result of more than 2^36 entries");
+    if (rows && g->n / rows_per_token > (1ull << 40) / width) return fail(DPB_EINVAL, "rows of more than 2^40 entries");
     const FwdDevice dev(ctx);
     DPB_CUDA(dev.err);
     return is_gl(family_dtype) ? sum_impl<GlFam>(ctx, g, weights, rows, rows_on_device, width, rows_per_token, multiplier, out)

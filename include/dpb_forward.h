@@ -55,8 +55,8 @@ void dpb_row_groups_free(dpb_row_groups* groups);
  * `weights`: a table of at least n challenge elements (an eq table of the row point, its entries past n unused) or
  * NULL for ones.  `rows`: an int64 row-major tensor of ceil(n / rows_per_token) x width entries, on the host or on the device, or NULL
  * for ones (width must be 1 then, and the sums are the weights' sums, or the number of rows).
- * The result is a table of 2^ceil(log2 n_keys) rows of 2^ceil(log2 width) entries, zero for keys without rows and
- * outside; its low variables are the columns. */
+ * The result is a table of 2^ceil(log2 n_keys) rows of 2^ceil(log2 width) entries (2^36 entries at most, of rows that
+ * hold 2^40 at most), zero for keys without rows and outside; its low variables are the columns. */
 int dpb_row_groups_sum(dpb_ctx* ctx, const dpb_row_groups* groups, int family_dtype, const dpb_mle* weights,
                        const int64_t* rows, int rows_on_device, uint64_t width, uint32_t rows_per_token,
                        int64_t multiplier, dpb_mle** out);

@@ -239,6 +239,23 @@ def test_groups_refusals(dpb, ctx, fw):
         g.sums(dpb.FR, rows=np.zeros((2, 4), np.int64))
 
 
+def test_row_sums_refuse_what_no_device_holds(dpb, ctx, fw):
+    """Sizes whose bytes would pass 64 bits further up are refused by their number, before anything is read or made."""
+    g = fw.RowGroups(ctx, np.zeros(512, np.int64), 1)
+    few = np.zeros(4, np.int64)
+    out = dpb.ctypes.c_void_p()
+    for width, per, match in ((2**32, 1, "rows of more than 2.40"), (2**32 + 1, 1, "1..2.32"), (2**31 + 1, 1, "rows of more than 2.40")):
+        with pytest.raises(dpb.DpbError, match=match) as e:
+            dpb.check(dpb.lib.dpb_row_groups_sum(ctx.h, g.h, dpb.FR, None, dpb.ctypes.c_void_p(few.ctypes.data), 0, width, per, 1,
+                                                 dpb.ctypes.byref(out)))
+        assert e.value.code == dpb.EINVAL
+    many = fw.RowGroups(ctx, np.zeros(3, np.int64), 2**22)
+    with pytest.raises(dpb.DpbError, match="result of more than 2.36"):
+        dpb.check(dpb.lib.dpb_row_groups_sum(ctx.h, many.h, dpb.FR, None, dpb.ctypes.c_void_p(few.ctypes.data), 0, 2**15, 1, 1,
+                                             dpb.ctypes.byref(out)))
+    assert g.sums(dpb.GL_EXT).to_host().reshape(-1).tolist() == [512, 0]  # the context works on
+
+
 @pytest.mark.parametrize("n_keys", [4, 5, 2048])
 @pytest.mark.parametrize("n,bad", [(3, [2]), (3000, range(0, 3000, 7)), (700, range(600)), (6000, [5999]), (5000, range(5000))])
 def test_bad_device_keys(dpb, ctx, fw, n_keys, n, bad):
