@@ -120,6 +120,9 @@ class State:
         if self.own:
             self.dpb, self.fwd = _package()
             self.ctx = _context()
+            # The program's torch work runs on the library's stream from here on: the calls return before their results
+            # are written, and what they free may still be read by work that is queued.
+            torch.cuda.set_stream(torch.cuda.ExternalStream(self.ctx.stream))
 
     def __del__(self):
         try:
