@@ -580,7 +580,9 @@ int dpb_trim(dpb_ctx* ctx) {
 int dpb_sync(dpb_ctx* ctx) {
     if (!ctx) return fail(DPB_EINVAL, "null context");
     DPB_CUDA(cudaStreamSynchronize(ctx->stream));
-    return DPB_OK;
+    const int rc = fwd_results_hold(ctx);
+    if (rc != DPB_OK) *fwd_gave_up_host(ctx) = 0;  // told: nothing older is under way
+    return rc;
 }
 
 void* dpb_stream(dpb_ctx* ctx) { return ctx ? (void*)ctx->stream : nullptr; }
@@ -843,7 +845,7 @@ int dpb_mle_to_host(const dpb_mle* mle, void* out, uint64_t len, int form) {
     }
     DPB_CUDA(cudaStreamSynchronize(ctx->stream));
     DPB_CUDA(cudaGetLastError());
-    return DPB_OK;
+    return fwd_results_hold(ctx);
 }
 
 uint64_t dpb_mle_len(const dpb_mle* mle) { return mle ? mle->len : 0; }
@@ -892,6 +894,7 @@ int dpb_mle_evaluate(dpb_ctx* ctx, const dpb_mle* mle, const void* point, uint32
             DPB_CUDA(cudaMemcpyAsync(narrow ? (void*)&x32 : (void*)&x, mle->ptr, narrow ? 4 : 8, cudaMemcpyDeviceToHost,
                                      ctx->stream));
             DPB_CUDA(cudaStreamSynchronize(ctx->stream));
+            DPB_TRY(fwd_results_hold(ctx));
             if (narrow) x = x32;
             if (is_gl(mle->dtype)) {
                 const uint64_t mag = x < 0 ? (uint64_t)0 - (uint64_t)x : (uint64_t)x;
@@ -908,11 +911,11 @@ int dpb_mle_evaluate(dpb_ctx* ctx, const dpb_mle* mle, const void* point, uint32
             DPB_CUDA(cudaMemcpyAsync(v, mle->ptr, 8, cudaMemcpyDeviceToHost, ctx->stream));
             DPB_CUDA(cudaStreamSynchronize(ctx->stream));
             memcpy(out, v, 16);
-            return DPB_OK;
+            return fwd_results_hold(ctx);
         }
         DPB_CUDA(cudaMemcpyAsync(out, mle->ptr, dtype_size(mle->dtype), cudaMemcpyDeviceToHost, ctx->stream));
         DPB_CUDA(cudaStreamSynchronize(ctx->stream));
-        return DPB_OK;
+        return fwd_results_hold(ctx);
     }
     dpb_mle* res = nullptr;
     DPB_TRY(fix_common(ctx, mle, point, n, false, &res));
@@ -998,7 +1001,7 @@ int dpb_mle_evaluate_many(dpb_ctx* ctx, dpb_mle* const* mles, uint32_t n, const 
         cudaError_t e = cudaGetLastError();
         if (e == cudaSuccess) e = cudaMemcpyAsync(out, d_out, (size_t)n * es, cudaMemcpyDeviceToHost, ctx->stream);
         if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
-        if (e != cudaSuccess) rc = fail(DPB_ECUDA, "evaluate many: %s", cudaGetErrorString(e));
+        rc = e != cudaSuccess ? fail(DPB_ECUDA, "evaluate many: %s", cudaGetErrorString(e)) : fwd_results_hold(ctx);
     }
     device_free(ctx, d_src);
     device_free(ctx, d_scale);

@@ -42,11 +42,6 @@ int fwd_slot_take(dpb_ctx* ctx) {
 
 int fwd_check_begin(dpb_ctx* ctx, FwdCheck* out, int slot) {
     DPB_TRY(fwd_init(ctx));
-    volatile unsigned int* gave_up = (volatile unsigned int*)ctx->fwd_host + 2;
-    if (*gave_up) {
-        *gave_up = 0;
-        return fail(DPB_ETIMEOUT, "a kernel of an earlier forward call gave up waiting; that call's result is not valid");
-    }
     out->words = ctx->fwd_words;
     out->status = (unsigned long long*)ctx->fwd_dev + (slot < 0 ? 0 : kSlotWord + slot);
     out->seq = ++ctx->fwd_seq;
@@ -352,7 +347,7 @@ extern "C" int dpb_embedding_lookup(dpb_ctx* ctx, const dpb_mle* table, uint64_t
     if (right_shift > 62) return fail(DPB_EINVAL, "right shift %u exceeds 62", right_shift);
     if (n > (1ull << 40) / pow2_ceil(width)) return fail(DPB_EINVAL, "a result of more than 2^40 entries");
     const FwdDevice dev(ctx);
-    DPB_CUDA(dev.err);
+    DPB_TRY(fwd_ready(ctx, dev));
     return lookup_impl(ctx, table, vocab, width, row_stride, tokens, tokens_on_device, n, multiplier, right_shift, padded, out);
 }
 
@@ -362,7 +357,7 @@ extern "C" int dpb_row_groups_new(dpb_ctx* ctx, const int64_t* keys, int keys_on
     if (n_keys < 1 || n_keys > (1ull << 22)) return fail(DPB_EINVAL, "%llu keys (1..2^22)", (unsigned long long)n_keys);
     if (n >= (1ull << 31)) return fail(DPB_EINVAL, "%llu rows (below 2^31)", (unsigned long long)n);
     const FwdDevice dev(ctx);
-    DPB_CUDA(dev.err);
+    DPB_TRY(fwd_ready(ctx, dev));
     dpb_row_groups* g = new (std::nothrow) dpb_row_groups();
     if (!g) return fail(DPB_ENOMEM, "host allocation failed");
     g->ctx = ctx;
@@ -406,7 +401,16 @@ extern "C" int dpb_row_groups_sum(dpb_ctx* ctx, const dpb_row_groups* g, int fam
     if (pow2_ceil(g->n_keys) * pow2_ceil(width) > (1ull << 36)) return fail(DPB_EINVAL, "a result of more than 2^36 entries");
     if (rows && g->n / rows_per_token > (1ull << 40) / width) return fail(DPB_EINVAL, "rows of more than 2^40 entries");
     const FwdDevice dev(ctx);
-    DPB_CUDA(dev.err);
+    DPB_TRY(fwd_ready(ctx, dev));
     return is_gl(family_dtype) ? sum_impl<GlFam>(ctx, g, weights, rows, rows_on_device, width, rows_per_token, multiplier, out)
                                : sum_impl<FrFam>(ctx, g, weights, rows, rows_on_device, width, rows_per_token, multiplier, out);
+}
+
+// Tests: the word as a kernel that gave up waiting leaves it.  Not part of the interface.
+extern "C" int dpb_forward_give_up(dpb_ctx* ctx) {
+    const FwdDevice dev(ctx);
+    DPB_TRY(fwd_ready(ctx, dev));
+    DPB_TRY(fwd_init(ctx));
+    *fwd_gave_up_host(ctx) = 1;
+    return DPB_OK;
 }

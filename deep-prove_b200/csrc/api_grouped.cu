@@ -152,7 +152,7 @@ extern "C" int dpb_expert_weights_new(dpb_ctx* ctx, const int64_t* weights, int 
         return fail(DPB_EINVAL, "%u matrices of %llu x %llu entries", n_experts, (unsigned long long)inner, (unsigned long long)cols);
     if (bits < 2 || bits > 15) return fail(DPB_EINVAL, "weights of %u bits (2..15)", bits);
     const FwdDevice dev(ctx);
-    DPB_CUDA(dev.err);
+    DPB_TRY(fwd_ready(ctx, dev));
     dpb_expert_weights* w = new (std::nothrow) dpb_expert_weights();
     if (!w) return fail(DPB_ENOMEM, "host allocation failed");
     w->ctx = ctx;
@@ -191,6 +191,6 @@ extern "C" int dpb_grouped_product(dpb_ctx* ctx, int family_dtype, const dpb_row
         return fail(DPB_EINVAL, "%llu routed rows are not a multiple of %u per token", (unsigned long long)g->n, rows_per_token);
     if (g->n > (1ull << 40) / w->cols) return fail(DPB_EINVAL, "a result of more than 2^40 entries");
     const FwdDevice dev(ctx);
-    DPB_CUDA(dev.err);
+    DPB_TRY(fwd_ready(ctx, dev));
     return product_impl(ctx, is_gl(family_dtype) ? DPB_GL_I64 : DPB_FR_I64, g, x, x_on_device, x_bits, rows_per_token, w, out);
 }

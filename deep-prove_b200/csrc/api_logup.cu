@@ -147,6 +147,7 @@ static int build_trees(dpb_ctx* ctx, const LogupSpec* specs, uint32_t n, dpb_log
             if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
         }
         if (e != cudaSuccess) rc = fail(DPB_ECUDA, "logup trees: %s", cudaGetErrorString(e));
+        else if (host_outputs) rc = fwd_results_hold(ctx);
     }
     device_free(ctx, d);
     return rc;
@@ -234,7 +235,7 @@ int dpb_logup_outputs(const dpb_logup* lu, void* out4) {
     DPB_CUDA(cudaMemcpyAsync(out4, lu->num[top - 1], 2 * es, cudaMemcpyDeviceToHost, ctx->stream));
     DPB_CUDA(cudaMemcpyAsync((char*)out4 + 2 * es, lu->den[top - 1], 2 * es, cudaMemcpyDeviceToHost, ctx->stream));
     DPB_CUDA(cudaStreamSynchronize(ctx->stream));
-    return DPB_OK;
+    return fwd_results_hold(ctx);
 }
 
 int dpb_logup_outputs_batch(const dpb_logup* const* lus, uint32_t n, void* out) {
@@ -258,7 +259,7 @@ int dpb_logup_outputs_batch(const dpb_logup* const* lus, uint32_t n, void* out) 
     if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
     device_free(ctx, gathered);
     if (e != cudaSuccess) return fail(DPB_ECUDA, "logup outputs: %s", cudaGetErrorString(e));
-    return DPB_OK;
+    return fwd_results_hold(ctx);
 }
 
 void dpb_logup_free(dpb_logup* lu) {

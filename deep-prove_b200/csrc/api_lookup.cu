@@ -131,6 +131,11 @@ static int witness_impl(dpb_ctx* ctx, const dpb_chunking_info& ci, int64_t fpm, 
         dpb_mle_free(owner);
         return fail(DPB_ECUDA, "lookup witness: %s", cudaGetErrorString(e));
     }
+    rc = fwd_results_hold(ctx);  // before the verdict on values that may come from such a result
+    if (rc != DPB_OK) {
+        dpb_mle_free(owner);
+        return rc;
+    }
     if (err_host) {
         dpb_mle_free(owner);
         return fail(DPB_EINVAL, "Input value out of range for SignedZeroCheckTable, min: -32768, max: 32767");
@@ -218,7 +223,7 @@ extern "C" int dpb_lookup_counts_to_host(const dpb_lookup_counts* c, uint64_t* o
     cudaError_t e = cudaMemcpyAsync(out, c->dev, len * 8, cudaMemcpyDeviceToHost, c->ctx->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(c->ctx->stream);
     if (e != cudaSuccess) return fail(DPB_ECUDA, "reading counters: %s", cudaGetErrorString(e));
-    return DPB_OK;
+    return fwd_results_hold(c->ctx);
 }
 
 extern "C" void dpb_lookup_counts_free(dpb_lookup_counts* c) {

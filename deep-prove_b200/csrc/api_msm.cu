@@ -811,6 +811,7 @@ int dpb_pcs_batch_commit(dpb_ctx* ctx, const dpb_g1_bases* bases, dpb_mle* const
         for (auto& job : jobs) device_free(ctx, job.slab);
         if (rc != DPB_OK) return rc;
         if (e != cudaSuccess) return fail(DPB_ECUDA, "msm: %s", cudaGetErrorString(e));
+        DPB_TRY(fwd_results_hold(ctx));
         memcpy((char*)out_affine_xy + (size_t)first * 64, xy.data(), (size_t)cnt * 64);
     }
     return DPB_OK;

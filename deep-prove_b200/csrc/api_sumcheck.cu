@@ -1766,6 +1766,7 @@ int dpb_sumcheck_round(dpb_sc* sc, const void* prev_challenge, void* out_evals, 
     } else {
         rc = dpb_sumcheck_round(sc->tail, prev_challenge, out_evals, nullptr);
     }
+    if (rc == DPB_OK) rc = fwd_results_hold(sc->ctx);
     if (rc != DPB_OK) return rc;
     if (n_evals) *n_evals = sc->d + 1;
     sc->global_round++;
@@ -1785,6 +1786,7 @@ int dpb_sumcheck_finish(dpb_sc* sc, const void* last_challenge, void* out_final_
                                           : tail_finish<FrFam>(sc, last_challenge, out_final_evals);
     else rc = sc->gl ? run_finish<GlFam>(sc, last_challenge, out_final_evals)
                      : run_finish<FrFam>(sc, last_challenge, out_final_evals);
+    if (rc == DPB_OK) rc = fwd_results_hold(sc->ctx);
     if (rc != DPB_OK) return rc;
     sc->finished = true;
     return DPB_OK;

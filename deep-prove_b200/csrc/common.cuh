@@ -217,6 +217,18 @@ inline ReduceScratch<F> reduce_scratch(const dpb_ctx* ctx) {
     return rs;
 }
 
+// A forward kernel whose wait ran out leaves a word behind in mapped memory (forward.cuh) and a result that is not
+// valid.  Calls that hand values to the host, or take new forward work, ask here once those values are there, and fail
+// until dpb_sync has said so.
+inline volatile unsigned int* fwd_gave_up_host(const dpb_ctx* ctx) {
+    return ctx->fwd_host ? (volatile unsigned int*)ctx->fwd_host + 2 : nullptr;
+}
+inline int fwd_results_hold(const dpb_ctx* ctx) {
+    const volatile unsigned int* word = fwd_gave_up_host(ctx);
+    if (!word || !*word) return DPB_OK;
+    return fail(DPB_ETIMEOUT, "a kernel of an earlier forward call gave up waiting; what was made from its result is not valid");
+}
+
 int device_alloc(dpb_ctx* ctx, size_t bytes, void** out);
 void device_free(dpb_ctx* ctx, void* p);
 // Queues a copy of a (small) host buffer to device memory on the context's stream and returns at once: the

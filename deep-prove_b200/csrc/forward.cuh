@@ -89,7 +89,13 @@ struct FwdDevice {
     }
 };
 
-// The next check of the context (api_forward.cu); DPB_ETIMEOUT when a kernel of an earlier call gave up waiting.  With a
+// What every forward call asks for before it does anything.
+inline int fwd_ready(const dpb_ctx* ctx, const FwdDevice& dev) {
+    DPB_CUDA(dev.err);
+    return fwd_results_hold(ctx);
+}
+
+// The next check of the context (api_forward.cu).  With a
 // slot (fwd_slot_take) the findings stay readable until the slot is given back; without one, until the next check.
 int fwd_check_begin(dpb_ctx* ctx, FwdCheck* out, int slot = -1);
 int fwd_slot_take(dpb_ctx* ctx);  // -1: none is free

@@ -97,7 +97,8 @@ int dpb_init(int device, dpb_ctx** out);
 int dpb_trim(dpb_ctx* ctx);
 void dpb_shutdown(dpb_ctx* ctx);
 const char* dpb_last_error(void);
-/* Blocks until all work queued on the context's stream has finished. */
+/* Blocks until all work queued on the context's stream has finished.  DPB_ETIMEOUT when a kernel of a forward call
+ * (dpb_forward.h) gave up a bounded wait since the last dpb_sync. */
 int dpb_sync(dpb_ctx* ctx);
 /* The context's CUDA stream (a cudaStream_t), for callers that time with
  * CUDA events or order their own copies against it. */
