@@ -468,7 +468,8 @@ __global__ void __launch_bounds__(kGroupedThreads, 1) grouped_product_kernel(Gro
             const uint64_t c = (uint64_t)it.col_tile * kTileCols + (warp & 3) * 32 + lane;
             TileRows<T> rows;
             rows.load(a.rows, lo, valid);
-            if (!bar_wait(acc_full(buf), buf_phase, &gave_up)) goto done;
+            // the lanes stay together: one of them may see the limit pass where another still sees the tile arrive
+            if (!__all_sync(0xffffffffu, bar_wait(acc_full(buf), buf_phase, &gave_up))) goto done;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             store_tile<S::kAcc, T>(a, tmem + buf * (S::kAcc * T) + ((warp & 3) << 21), rows, valid, c, warp >> 2,
                                    [&]() { if (lane == 0) bar_arrive(acc_empty(buf)); });
