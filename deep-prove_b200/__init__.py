@@ -8,6 +8,7 @@ but creating a Context raises when no CUDA device is usable, and a missing
 library raises at import.
 """
 import ctypes
+import math
 import os
 
 import numpy as np
@@ -463,7 +464,7 @@ class Mle:
     """A multilinear table on the device (dpb_mle)."""
 
     def __init__(self, ctx, h):
-        self.ctx, self.h = ctx, h
+        self.ctx, self.h, self._words = ctx, h, None
 
     @property
     def len(self):
@@ -476,6 +477,20 @@ class Mle:
     @property
     def device_ptr(self):
         return lib.dpb_mle_device_ptr(self.h)
+
+    def tensor_ptr(self, shape):
+        """The device address of an int64 tensor of this shape that lies in the table; ValueError when the table was
+        freed, has entries of another size or fewer of them.  What a handle stands for does not change: asked once."""
+        if not self.h:
+            raise ValueError("a device tensor that was freed")
+        if self._words is None:
+            self._words = (self.device_ptr, self.len if self.dtype in (GL_BASE, GL_I64, FR_I64) else -1)
+        ptr, n = self._words
+        if n < 0:
+            raise ValueError(f"a device tensor has 8-byte entries, not those of dtype {self.dtype}")
+        if math.prod(shape) > n or min(shape, default=0) < 0:
+            raise ValueError(f"a device tensor of shape {tuple(shape)} in a table of {n} entries")
+        return ptr
 
     def to_host(self, form=FORM_NATIVE, n=None):
         n = self.len if n is None else n

@@ -1,6 +1,7 @@
 """Python face of include/dpb_forward.h: the forward operators that make the integer tensors the provers take, and their
 transposes.  Device tensors are (table, shape) pairs, as Context.upload_tensor_i64 returns them; results of that form can
-be handed to the einsum and lookup calls' device_tensor arguments."""
+be handed to the einsum and lookup calls' device_tensor arguments.  A pair whose table was freed, has entries of another
+size than 8 bytes or fewer of them than the shape is a ValueError."""
 import ctypes
 import math
 
@@ -29,7 +30,7 @@ def _source(array, device):
     """(pointer, 1 when on the device, shape, what must stay alive) of an int64 tensor given either way."""
     if device is not None:
         mle, shape = device
-        return lib.dpb_mle_device_ptr(mle.h), 1, shape, mle
+        return mle.tensor_ptr(shape), 1, shape, mle
     a = np.ascontiguousarray(array, dtype=np.int64)
     return _buf(a), 0, a.shape, a
 
