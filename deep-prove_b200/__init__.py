@@ -357,7 +357,7 @@ class Context:
         views = (ctypes.c_void_p * cap)()
         owner = ctypes.c_void_p()
         n = ctypes.c_uint32()
-        src = _buf(t) if t is not None else ctypes.c_void_p(lib.dpb_mle_device_ptr(mle.h))
+        src = _buf(t) if t is not None else ctypes.c_void_p(mle.tensor_ptr(tshape))
         check(lib.dpb_einsum_fix_axes(self.h, family_dtype, src, 0 if t is not None else 1, shape, kd, pts, lens, rank,
                                       ctypes.byref(owner), views, cap, ctypes.byref(n)))
         return Mle(self, owner), [Mle(self, ctypes.c_void_p(views[i])) for i in range(n.value)]
@@ -424,7 +424,7 @@ def lookup_witness(ctx, family_dtype, info, fixed_point_multiplier, padding_valu
     Returns (owner, input columns, output columns)."""
     if device_tensor is not None:
         mle, tshape = device_tensor
-        src, on_dev = ctypes.c_void_p(lib.dpb_mle_device_ptr(mle.h)), 1
+        src, on_dev = ctypes.c_void_p(mle.tensor_ptr(tshape)), 1
     else:
         t = np.ascontiguousarray(tensor, dtype=np.int64)
         tshape, src, on_dev = t.shape, _buf(t), 0
@@ -438,7 +438,7 @@ def lookup_witness(ctx, family_dtype, info, fixed_point_multiplier, padding_valu
     n_in, n_out, owner = ctypes.c_uint32(), ctypes.c_uint32(), ctypes.c_void_p()
     tab = None if value_table_outputs is None else np.ascontiguousarray(value_table_outputs, dtype=np.int64)
     if device_table is not None:
-        tab_ptr, tab_dev = ctypes.c_void_p(lib.dpb_mle_device_ptr(device_table[0].h)), 1
+        tab_ptr, tab_dev = ctypes.c_void_p(device_table[0].tensor_ptr(device_table[1])), 1
     else:
         tab_ptr, tab_dev = (_buf(tab) if tab is not None else None), 0
     hs = [c.h if c is not None else None for c in counts]

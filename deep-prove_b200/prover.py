@@ -416,7 +416,7 @@ class EinsumOperand:
         if device_tensor is not None:
             mle, shape = device_tensor
             self._keep = [mle]
-            self.ptr, self.on_device = lib.dpb_mle_device_ptr(mle.h), 1
+            self.ptr, self.on_device = mle.tensor_ptr(shape), 1
         else:
             t = np.ascontiguousarray(tensor, dtype=np.int64)
             shape = t.shape

@@ -95,6 +95,26 @@ def test_a_table_of_other_entries_or_freed(dpb, fw, shape):
         assert fw.Fake.reached is None
 
 
+@pytest.mark.parametrize("shape,dtype,freed", [((3, 6), "GL_BASE", False), ((2, 4), "FR", False), ((2, 4), "FR_I64", True)])
+def test_the_calls_that_take_such_results(dpb, fw, shape, dtype, freed):
+    """The einsum and lookup calls' device tensors are held to the same."""
+    prover = importlib.import_module("deep_prove_b200.prover")
+    mle = dpb.Mle(Ctx(), FakeTable(getattr(dpb, dtype), 16))
+    if freed:
+        mle.free()
+    ctx = dpb.Context.__new__(dpb.Context)
+    ctx.h = None
+    kinds, info, x = (dpb.AXIS_OUTER, dpb.AXIS_CONTRACTED), dpb.ChunkingInfo(), np.zeros((2, 2), np.int64)
+    for call in (lambda: ctx.einsum_fix_axes(dpb.FR, None, kinds, [None, None], device_tensor=(mle, shape)),
+                 lambda: prover.EinsumOperand(None, kinds, [None, None], device_tensor=(mle, shape)),
+                 lambda: dpb.lookup_witness(ctx, dpb.FR, info, 1, 0, None, None, 1, device_tensor=(mle, shape)),
+                 lambda: dpb.lookup_witness(ctx, dpb.FR, info, 1, 0, x, None, 2, device_table=(mle, shape))):
+        fw.Fake.reached = None
+        with pytest.raises(ValueError, match="device tensor"):
+            call()
+        assert fw.Fake.reached is None
+
+
 def test_negative_extents(dpb, fw):
     for call in calls(dpb, fw, (dpb.Mle(Ctx(), FakeTable(dpb.FR_I64, 16)), (-2, -3))):
         with pytest.raises(ValueError):
