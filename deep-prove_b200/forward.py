@@ -74,6 +74,8 @@ class RowGroups:
             if len(shape) != 2 or shape[0] < -(-self.n // rows_per_token):
                 raise ValueError(f"rows of shape {shape} for {self.n} keys, {rows_per_token} per token")
             width = shape[1]
+        if weights is not None and not weights.h:
+            raise ValueError("weights that were freed")
         h = ctypes.c_void_p()
         check(lib.dpb_row_groups_sum(self.ctx.h, self.h, family_dtype, weights.h if weights is not None else None, ptr, on_device,
                                      width, rows_per_token, multiplier, ctypes.byref(h)))

@@ -95,6 +95,18 @@ def test_a_table_of_other_entries_or_freed(dpb, fw, shape):
         assert fw.Fake.reached is None
 
 
+def test_freed_weights_are_not_ones(dpb, fw):
+    """The library takes no weights for ones."""
+    w = dpb.Mle(Ctx(), FakeTable(dpb.FR, 8))
+    groups_of(fw, 5).sums(dpb.FR, weights=w)
+    w.free()
+    for rows in (None, np.ones((5, 2), np.int64)):
+        fw.Fake.reached = None
+        with pytest.raises(ValueError, match="freed"):
+            groups_of(fw, 5).sums(dpb.FR, weights=w, rows=rows)
+        assert fw.Fake.reached is None
+
+
 @pytest.mark.parametrize("shape,dtype,freed", [((3, 6), "GL_BASE", False), ((2, 4), "FR", False), ((2, 4), "FR_I64", True)])
 def test_the_calls_that_take_such_results(dpb, fw, shape, dtype, freed):
     """The einsum and lookup calls' device tensors are held to the same."""
