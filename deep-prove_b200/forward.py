@@ -35,6 +35,18 @@ def _source(array, device):
     return _buf(a), 0, a.shape, a
 
 
+def _fit(bits, **values):
+    """The library's integer arguments have fixed widths, and ctypes would cut what does not fit."""
+    for name, v in values.items():
+        if not 0 <= v < 1 << bits:
+            raise ValueError(f"{name} {v} does not fit {bits} bits")
+
+
+def _fit_signed(multiplier):
+    if not -(1 << 63) <= multiplier < 1 << 63:
+        raise ValueError(f"multiplier {multiplier} does not fit 64 bits")
+
+
 def _pow2(n):
     return 1 << (max(int(n), 1) - 1).bit_length()
 
@@ -44,10 +56,14 @@ def embedding_lookup(ctx, table, vocab, width, tokens, multiplier=1, right_shift
     """dpb_embedding_lookup: the rows of `tokens`, rescaled.  `table`: an integer table of vocab rows, row_stride
     (default: width) entries apart.  Returns (table, shape): the [n, width] tensor, or with padded=True the table of
     the padded shape."""
+    row_stride = width if row_stride is None else row_stride
+    _fit(64, vocab=vocab, width=width, row_stride=row_stride)
+    _fit(32, right_shift=right_shift)
+    _fit_signed(multiplier)
     ptr, on_device, shape, _keep = _source(tokens, device_tokens)
     n = math.prod(shape)
     h = ctypes.c_void_p()
-    check(lib.dpb_embedding_lookup(ctx.h, table.h, vocab, width, width if row_stride is None else row_stride, ptr, on_device, n,
+    check(lib.dpb_embedding_lookup(ctx.h, table.h, vocab, width, row_stride, ptr, on_device, n,
                                    multiplier, right_shift, 1 if padded else 0, ctypes.byref(h)))
     return Mle(ctx, h), (_pow2(n), _pow2(width)) if padded else (n, width)
 
@@ -58,6 +74,7 @@ class RowGroups:
 
     def __init__(self, ctx, keys, n_keys, device_keys=None):
         self.ctx, self.h = ctx, None
+        _fit(64, n_keys=n_keys)
         ptr, on_device, shape, _keep = _source(keys, device_keys)
         self.n, self.n_keys = math.prod(shape), int(n_keys)
         h = ctypes.c_void_p()
@@ -67,11 +84,13 @@ class RowGroups:
     def sums(self, family_dtype, weights=None, rows=None, rows_per_token=1, multiplier=1, device_rows=None):
         """dpb_row_groups_sum: out[k, c] = multiplier * sum over rows i with key k of weights[i] * rows[i //
         rows_per_token, c], a table of the padded shape over the family's challenge elements."""
+        _fit(32, rows_per_token=rows_per_token)
+        _fit_signed(multiplier)
         if rows is None and device_rows is None:
             ptr, on_device, width = None, 0, 1
         else:
             ptr, on_device, shape, _keep = _source(rows, device_rows)
-            if len(shape) != 2 or shape[0] < -(-self.n // rows_per_token):
+            if len(shape) != 2 or shape[0] < -(-self.n // max(rows_per_token, 1)):
                 raise ValueError(f"rows of shape {shape} for {self.n} keys, {rows_per_token} per token")
             width = shape[1]
         if weights is not None and not weights.h:
@@ -92,6 +111,7 @@ class ExpertWeights:
 
     def __init__(self, ctx, weights, bits, device_weights=None):
         self.ctx, self.h = ctx, None
+        _fit(32, bits=bits)
         ptr, on_device, shape, _keep = _source(weights, device_weights)
         if len(shape) != 3:
             raise ValueError(f"weights of shape {shape}: [expert, in, out] expected")
@@ -109,6 +129,7 @@ class ExpertWeights:
 def grouped_product(ctx, groups, x, x_bits, weights, rows_per_token=1, device_x=None, family_dtype=FR_I64):
     """dpb_grouped_product: row i of x[i // rows_per_token] times its expert's matrix, exact.  Returns (table, shape) of
     the [rows, out] tensor, rows in the order of the groups' keys."""
+    _fit(32, x_bits=x_bits, rows_per_token=rows_per_token)
     ptr, on_device, shape, _keep = _source(x, device_x)
     if len(shape) != 2 or shape[1] != weights.inner or shape[0] * rows_per_token != groups.n:
         raise ValueError(f"x of shape {shape} for {groups.n} routed rows, {rows_per_token} per token, of {weights.inner} entries")

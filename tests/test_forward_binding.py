@@ -107,6 +107,30 @@ def test_freed_weights_are_not_ones(dpb, fw):
         assert fw.Fake.reached is None
 
 
+def test_integers_that_the_arguments_cannot_hold(dpb, fw):
+    """2^32 + 1 rows per token would arrive as 1 row, 2^63 times as -2^63 times."""
+    table, tokens, x = dpb.Mle(Ctx(), FakeTable(dpb.FR_I32, 64)), np.zeros(3, np.int64), np.ones((3, 2), np.int64)
+    w = fw.ExpertWeights(Ctx(), np.ones((4, 2, 5), np.int64), 8)
+    lookup = lambda **kw: fw.embedding_lookup(Ctx(), table, **{**dict(vocab=8, width=8, tokens=tokens), **kw})
+    for call in (lambda: lookup(multiplier=2**63), lambda: lookup(multiplier=-2**63 - 1), lambda: lookup(right_shift=2**32),
+                 lambda: lookup(right_shift=-1), lambda: lookup(vocab=2**64 + 1), lambda: lookup(row_stride=2**64 + 8),
+                 lambda: lookup(width=-8), lambda: fw.RowGroups(Ctx(), tokens, 2**64 + 4),
+                 lambda: groups_of(fw, 3).sums(dpb.FR, rows=x, rows_per_token=2**32 + 1),
+                 lambda: groups_of(fw, 3).sums(dpb.FR, multiplier=2**63),
+                 lambda: fw.ExpertWeights(Ctx(), np.ones((4, 2, 5), np.int64), 2**32 + 8),
+                 lambda: fw.grouped_product(Ctx(), groups_of(fw, 3), x, 2**32 + 8, w)):
+        fw.Fake.reached = None
+        with pytest.raises(ValueError, match="does not fit"):
+            call()
+        assert fw.Fake.reached is None
+    # the library itself refuses none per token, with rows as well
+    for kw in (dict(), dict(rows=x)):
+        groups_of(fw, 3).sums(dpb.FR, rows_per_token=0, **kw)
+        assert fw.Fake.reached[0] == "dpb_row_groups_sum" and fw.Fake.reached[1][7] == 0
+    lookup(multiplier=-2**63, right_shift=62)
+    assert fw.Fake.reached[1][8:10] == (-2**63, 62)
+
+
 @pytest.mark.parametrize("shape,dtype,freed", [((3, 6), "GL_BASE", False), ((2, 4), "FR", False), ((2, 4), "FR_I64", True)])
 def test_the_calls_that_take_such_results(dpb, fw, shape, dtype, freed):
     """The einsum and lookup calls' device tensors are held to the same."""
