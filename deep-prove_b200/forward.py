@@ -35,11 +35,11 @@ def _source(array, device):
     return _buf(a), 0, a.shape, a
 
 
-def _fit(bits, **values):
+def _fit(size, /, **values):
     """The library's integer arguments have fixed widths, and ctypes would cut what does not fit."""
     for name, v in values.items():
-        if not 0 <= v < 1 << bits:
-            raise ValueError(f"{name} {v} does not fit {bits} bits")
+        if not 0 <= v < 1 << size:
+            raise ValueError(f"{name} {v} does not fit {size} bits")
 
 
 def _fit_signed(multiplier):
