@@ -89,9 +89,13 @@ struct FwdDevice {
     }
 };
 
-// What every forward call asks for before it does anything.
+// What every forward call asks for before it does anything.  Inside a capture of the stream a check's findings would
+// never come, and a replay would write into scratch memory that has been handed on since.
 inline int fwd_ready(const dpb_ctx* ctx, const FwdDevice& dev) {
     DPB_CUDA(dev.err);
+    cudaStreamCaptureStatus capture;
+    DPB_CUDA(cudaStreamIsCapturing(ctx->stream, &capture));
+    if (capture != cudaStreamCaptureStatusNone) return fail(DPB_ESTATE, "forward calls are made outside captures of the context's stream");
     return fwd_results_hold(ctx);
 }
 

@@ -13,8 +13,8 @@
  *
  * Conventions are those of dpb.h.  Work is queued on the context's stream (dpb_stream); device inputs must be ready on
  * that stream and stay as they are until it has passed the call, and results are ready on it.  Calls that check values
- * on the device wait for that check before they return, so they cannot be made inside a stream capture; their results
- * may still be in the making.  Waits inside kernels are bounded.  When one runs out, the result is not valid, which may
+ * on the device wait for that check before they return; their results may still be in the making.  None of the calls
+ * can be made while the context's stream is being captured (DPB_ESTATE, and the capture goes on).  Waits inside kernels are bounded.  When one runs out, the result is not valid, which may
  * show after the call has returned: from then on the calls here, and every call that hands values to the host
  * (dpb_mle_to_host, evaluations, sumcheck rounds and the provers, logup outputs, counters, commitments), fail with
  * DPB_ETIMEOUT until dpb_sync has reported it; what was made from results older than that is to be made again.
