@@ -53,6 +53,11 @@ class TransformerShape:
     experts: int = 0             # routed feed-forward layers: so many matrices (a power of two), 0 for dense ones
     experts_per_token: int = 2
 
+    def __post_init__(self):
+        if self.experts and (self.glu or self.experts & (self.experts - 1) or not 1 <= self.experts_per_token <= self.experts):
+            raise ValueError(f"{self.name}: routed layers take a power of two of matrices, at least as many as a token's, and "
+                             "no gated part")
+
 
 @dataclass(frozen=True)
 class MlpShape:
