@@ -2,8 +2,6 @@
 integers.  TEST INFRASTRUCTURE ONLY, like the rest of oracle/."""
 import numpy as np
 
-from . import oracle as orc
-
 
 def pow2(n):
     return 1 << (max(int(n), 1) - 1).bit_length()
@@ -46,7 +44,3 @@ def grouped_product(x, keys, weights, rows_per_token=1):
     for i, k in enumerate(keys):
         out[i] = x[i // rows_per_token].astype(np.int64) @ weights[k].astype(np.int64)
     return out
-
-
-def table_of(F, scalars):
-    return orc.scalars_to_array(F, scalars)
