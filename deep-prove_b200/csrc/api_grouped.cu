@@ -78,8 +78,14 @@ static int product_impl(dpb_ctx* ctx, int dtype, const dpb_row_groups* g, const 
     // Rows per tile.  An instruction takes as long for 16 rows as for 128 (about 70 clocks; 85 for 160), so a tile should
     // hold what an expert gets: fewer, fuller tiles read the weights less often.  Small tiles leave room for more stages
     // (few rows: bound by the weights' way from HBM) and, up to 64 rows of two digits, for a second accumulator.
-    // Measured: 52 rows per expert 24.9 us with 64, 25.9 with 128; 128 rows 68 us the call with 128, 73 with 80, 72 with 96;
-    // 2048 rows 1.95 ms with 160, 2.04 with 128, 3.4 with 64.
+    // The average stands for all experts: their counts stay on the device.
+    // Measured, the whole call in us, 8 experts of 2048 x 4096, 14 x 12 bits, balanced routes / routes that prefer some
+    // experts: 8 rows per expert 30/31 with 16, 32/32 with 32; 12 rows 31/39 with 16, 31/31 with 32, 33/33 with 64; 16 rows
+    // 32/32 with 32, 34/34 with 64; 24 rows 32/42 with 32, 33/34 with 64; 48 rows 34/42 with 64, 39/40 with 128; 64 rows
+    // 36/44 with 64, 41/42 with 128; 80 rows 53/53 with 64, 44/44 with 128.  Between 128 and 160 it goes by how the counts
+    // fill whole tiles until they are large (experts of 4096 x 11008): 256 rows 324/420 with 128, 372/354 with 160; 320
+    // rows 464/462 and 405/465; 512 rows 628/689 and 724/684; 1024 rows 1234/1291 and 1234/1211; 2048 rows 2389/2468 and
+    // 2255/2298; with 8 x 8 bits 512 rows 294/311 and 331/310, 2048 rows 1076/1094 and 1022/1038.
     const uint64_t used = std::min<uint64_t>(w->n_experts, n), average = (n + used - 1) / used;
     const uint32_t T = average <= 8 ? 16 : average <= 16 ? 32 : average <= 64 ? 64 : average < 320 ? 128 : 160;
     const uint64_t max_tiles = n / T + used;  // every expert's last tile may be partly filled

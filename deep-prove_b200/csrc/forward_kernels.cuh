@@ -39,7 +39,8 @@ __device__ __forceinline__ int64_t lookup_scale(const LookupArgs& a, int64_t x, 
 // wherever they suffice, since finding a step's row takes a division (by a multiplication then).  kLookupFlight steps per thread are under way
 // together: tokens, then table entries, then results; steps of neighbouring threads are neighbours, and a thread's own
 // lie a grid apart (next to each other they fill fewer blocks of a short call: 8 us instead of 5).  16384 rows of 4096
-// entries of 8 bytes take 168 us: 1.07 GB, 4.3 TB/s of it from and to HBM and the rest rows that several tokens share.
+// entries of 8 bytes take 168 us: 1.07 GB, of which 0.74 GB from and to HBM (4.4 TB/s) and the rest rows that several
+// tokens share.  Neither HBM (57 %) nor the instructions' issue (60 %) is full; the registers hold 46 % of an SM's warps.
 constexpr int kLookupFlight = 4;
 template <class T, int V, bool CHECK, class I>
 __global__ void __launch_bounds__(kLookupThreads, sizeof(I) == 4 ? 4 : 2) embedding_lookup_kernel(LookupArgs a) {
@@ -375,8 +376,8 @@ __device__ __forceinline__ void clear_unsummed(const RowSumArgs& a) {
 // a double, a product is at most 2^47 and kExactRows of them stay within 2^53: the sums run as one fused multiply-add per
 // word on the 64-bit floating-point pipe, exactly, and move to signed 64-bit integers every kExactRows rows.  Wide integer
 // multiply-adds run at half a double's rate, and came with as many moves: 8192 rows of 4096 over BN254 took 88 us in a
-// chain of carries, 76 us in one 64-bit accumulator per word, and take 59 us this way.  What bounds it then is shared
-// between the weights' and entries' way through shared memory (57 % of its wavefronts) and the instructions' issue (59 %).
+// chain of carries, 76 us in one 64-bit accumulator per word, and take 58 us this way.  What bounds it then is shared
+// between the weights' and entries' way through shared memory (64 % of its wavefronts) and the instructions' issue (53 %).
 // What an entry has above 16 bits, as quantised activations do not, takes a field product.
 constexpr uint32_t kExactRows = 64;
 constexpr uint64_t kRowSumMaxSlice = 49152;  // rows per slice: 2^47 times as many stays below 2^63
@@ -450,13 +451,13 @@ __device__ __noinline__ typename F::E add_high(typename F::E v, const typename F
     return hi < 0 ? F::sub(v, t) : F::add(v, t);
 }
 
-// A block: neighbouring columns of one slice.  Rows come in batches whose weights, and the weights'
-// prefix sums, go through shared memory; kRowSumFlight rows' entries are loaded ahead of the products.
+// A block: neighbouring columns of one slice.  Rows come in batches whose places and run ends, and weights, go through
+// shared memory.  Without weights a thread loads kRowSumFlight rows' entries ahead of the sums.
 constexpr uint32_t kRowSumThreads = 128, kRowSumBatch = 64, kRowSumFlight = 8;
 
 // With weights: two columns per thread (a weight read from shared memory then serves two products).  The entries come
 // through a per-thread ring in shared memory, kRingAhead groups of eight rows ahead of the products, so that loads are
-// under way all the time (groups of four, three ahead: 64.5 us where these take 61.5).
+// under way all the time (groups of four, three ahead: 3 us more over BN254, 8192 rows of 4096).
 constexpr uint32_t kRowRing = 2, kRingAhead = kRowRing - 1, kProductBatch = 128, kGroup = 8;
 template <int BYTES>
 __device__ __forceinline__ void ring_load(void* dst, const void* src) {
@@ -465,7 +466,7 @@ __device__ __forceinline__ void ring_load(void* dst, const void* src) {
     else
         asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
-// blocks per SM that the registers are held down for (BN254: 65 us with four, 68 with three and no spills)
+// blocks per SM that the registers are held down for (BN254, 8192 rows of 4096: 3 us more with three, which spill nothing)
 template <class F>
 constexpr int kProductBlocks = sizeof(typename F::E) == 32 ? 4 : 5;
 // PAIRS: rows of an even number of entries at 16-byte addresses, so that a thread's two columns are one word

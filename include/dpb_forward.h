@@ -46,7 +46,7 @@ int dpb_embedding_lookup(dpb_ctx* ctx, const dpb_mle* table, uint64_t vocab, uin
  * the calls below.  Keys are int64 in 0..n_keys-1; 1 <= n_keys <= 2^22, n < 2^31 (0 allowed).  Results do not depend
  * on the order of the rows inside a key.  DPB_EINVAL when a key lies outside the range: from this call for keys on the
  * host, from the first call that uses the rows (and every later one) for keys on the device, which are checked there
- * while the host goes on. */
+ * while the host goes on (or from this call, when 64 handles' checks are waiting to be asked for). */
 typedef struct dpb_row_groups dpb_row_groups;
 int dpb_row_groups_new(dpb_ctx* ctx, const int64_t* keys, int keys_on_device, uint64_t n, uint64_t n_keys,
                        dpb_row_groups** out);
