@@ -1742,6 +1742,14 @@ int dpb_sumcheck_begin_partial(dpb_ctx* ctx, uint32_t num_vars, dpb_mle* const* 
     return DPB_OK;
 }
 
+// Values of a round or the end that may come from a result that is not valid are not handed out, and the sumcheck, which
+// has gone on by then, takes no further call but dpb_sumcheck_free.
+static int held(dpb_sc* sc) {
+    const int rc = fwd_results_hold(sc->ctx);
+    if (rc != DPB_OK) sc->finished = true;
+    return rc;
+}
+
 int dpb_sumcheck_round(dpb_sc* sc, const void* prev_challenge, void* out_evals, uint32_t* n_evals) {
     if (!sc || !out_evals) return fail(DPB_EINVAL, "null argument");
     if (sc->merged) {
@@ -1766,7 +1774,7 @@ int dpb_sumcheck_round(dpb_sc* sc, const void* prev_challenge, void* out_evals, 
     } else {
         rc = dpb_sumcheck_round(sc->tail, prev_challenge, out_evals, nullptr);
     }
-    if (rc == DPB_OK) rc = fwd_results_hold(sc->ctx);
+    if (rc == DPB_OK) rc = held(sc);
     if (rc != DPB_OK) return rc;
     if (n_evals) *n_evals = sc->d + 1;
     sc->global_round++;
@@ -1786,7 +1794,7 @@ int dpb_sumcheck_finish(dpb_sc* sc, const void* last_challenge, void* out_final_
                                           : tail_finish<FrFam>(sc, last_challenge, out_final_evals);
     else rc = sc->gl ? run_finish<GlFam>(sc, last_challenge, out_final_evals)
                      : run_finish<FrFam>(sc, last_challenge, out_final_evals);
-    if (rc == DPB_OK) rc = fwd_results_hold(sc->ctx);
+    if (rc == DPB_OK) rc = held(sc);
     if (rc != DPB_OK) return rc;
     sc->finished = true;
     return DPB_OK;

@@ -113,6 +113,48 @@ def test_a_prover_and_a_commitment_say_so(dpb, give_up):
         ctx.close()
 
 
+@pytest.mark.parametrize("num_vars", [3, 6, 14])
+@pytest.mark.parametrize("at", [0, 1, 2])
+def test_a_sumcheck_that_was_told_goes_no_further(dpb, give_up, num_vars, at):
+    """Its rounds have gone on when the call fails: nothing but freeing it is left, also after the sync."""
+    F = orc.FrField
+    ctx = dpb.Context(0)
+    try:
+        rng = np.random.default_rng(5)
+        tabs = [ctx.upload_ints(rng.integers(-50, 50, size=1 << num_vars), dpb.FR_I32) for _ in range(2)]
+        r = orc.scalars_to_array(F, [F.random_scalar(rng)])
+        sc = ctx.sumcheck(num_vars, tabs, dpb.make_terms([(F.one, [0, 1])], F.to_native))
+        for i in range(at):
+            sc.round(r if i else None)
+        give_up(ctx)
+        with pytest.raises(dpb.DpbError, match="gave up waiting"):
+            sc.round(r if at else None)
+        with pytest.raises(dpb.DpbError, match="gave up waiting"):
+            ctx.sync()
+        for _ in range(num_vars + 2):
+            for call in (lambda: sc.round(r if at else None), lambda: sc.round(r), lambda: sc.finish(r)):
+                with pytest.raises(dpb.DpbError) as e:
+                    call()
+                assert e.value.code == dpb.ESTATE
+        sc.free()
+        # and at its end
+        sc = ctx.sumcheck(num_vars, tabs, dpb.make_terms([(F.one, [0, 1])], F.to_native))
+        for i in range(num_vars):
+            sc.round(r if i else None)
+        give_up(ctx)
+        with pytest.raises(dpb.DpbError, match="gave up waiting"):
+            sc.finish(r)
+        with pytest.raises(dpb.DpbError, match="gave up waiting"):
+            ctx.sync()
+        with pytest.raises(dpb.DpbError) as e:
+            sc.finish(r)
+        assert e.value.code == dpb.ESTATE
+        sc.free()
+        assert tabs[0].to_host(n=1).size == 1
+    finally:
+        ctx.close()
+
+
 def test_other_contexts_are_not_concerned(dpb, ctx, give_up):
     other = dpb.Context(0)
     try:
