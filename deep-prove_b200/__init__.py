@@ -488,7 +488,7 @@ class Mle:
         ptr, n = self._words
         if n < 0:
             raise ValueError(f"a device tensor has 8-byte entries, not those of dtype {self.dtype}")
-        if math.prod(shape) > n or (shape and min(shape) < 0):
+        if math.prod(map(int, shape)) > n or (len(shape) and min(shape) < 0):
             raise ValueError(f"a device tensor of shape {tuple(shape)} in a table of {n} entries")
         return ptr
 

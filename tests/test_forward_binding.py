@@ -151,6 +151,14 @@ def test_the_calls_that_take_such_results(dpb, fw, shape, dtype, freed):
         assert fw.Fake.reached is None
 
 
+def test_extents_that_numpy_would_cut(dpb, fw):
+    """2^40 * 2^24 = 2^64 is 0 in 64 bits."""
+    shape = (np.int64(2**40), np.int64(2**24))
+    for call in calls(dpb, fw, (dpb.Mle(Ctx(), FakeTable(dpb.FR_I64, 16)), shape))[1:2]:
+        with pytest.raises(ValueError, match="in a table of 16"):
+            call()
+
+
 def test_negative_extents(dpb, fw):
     for call in calls(dpb, fw, (dpb.Mle(Ctx(), FakeTable(dpb.FR_I64, 16)), (-2, -3))):
         with pytest.raises(ValueError):
